@@ -437,6 +437,43 @@ typedef struct mindiesd_rope_args {
 int mindiesd_rope(const mindiesd_rope_args* args, void* stream);
 
 /*
+ * Residual addition, root-mean-square norm and per-token quantisation of [rows, dim] activations:
+ *   v = x + residual (fp32),  y = v * weight / sqrt(mean(v^2) + eps)  (fp32)
+ *   out          = y rounded once to the type of x, or e4m3 of y / scale (out_dtype = MINDIESD_E4M3)
+ *   scales       fp32 [rows], e4m3 only: max|y| / 448 of the row (at least 2^-126), 1 for a row of zeros;
+ *                real value = stored value * scale.  A NaN or infinity in a row makes its scale NaN
+ *   residual_out = v rounded once to the residual's type; required exactly when residual is given
+ * x, residual: rows x_stride / residual_stride elements apart, channels contiguous; weight (NULL = ones):
+ * [dim]; out and residual_out: contiguous [rows, dim].  Any dim and any alignment of the element's size;
+ * 16-byte aligned rows are fastest.  residual and weight are in the type of x or fp32, each on its own.
+ * quant_only != 0: y = x (no norm; weight and residual must be NULL, out_dtype MINDIESD_E4M3; with an
+ * infinity in a row its scale is infinity).
+ *
+ * Stands in for RMSNorm of mindiesd/layers/norm.py with the residual addition before it, and for the
+ * dynamic per-token quantisation in front of the quantised linear layers of mindiesd/quantization/layer.py.
+ */
+typedef struct mindiesd_norm_args {
+    const void* x;
+    const void* residual;
+    const void* weight;
+    void* out;
+    void* residual_out;
+    float* scales;
+    int64_t rows;
+    int64_t x_stride;
+    int64_t residual_stride;
+    int32_t dim;
+    int32_t dtype;          /* MINDIESD_BF16 / FP16 / FP32 */
+    int32_t residual_dtype; /* dtype or MINDIESD_FP32 */
+    int32_t weight_dtype;   /* dtype or MINDIESD_FP32 */
+    int32_t out_dtype;      /* dtype or MINDIESD_E4M3 */
+    int32_t quant_only;
+    float eps;              /* > 0 */
+} mindiesd_norm_args;
+
+int mindiesd_add_rms_norm(const mindiesd_norm_args* args, void* stream);
+
+/*
  * The re-shard step of Ulysses sequence parallelism as one data-movement kernel.
  *
  * A rank holds `rows` tokens with all N heads: tensors [rows, N, 128] addressed by a row and a head

@@ -807,6 +807,80 @@ at::Tensor fp8_attention_cuda(const at::Tensor& query, const at::Tensor& key, co
     return out;
 }
 
+// ---- residual addition + RMS norm (+ per-token e4m3 quantisation) -------------------------------------------
+// A [..., D] tensor as rows of D contiguous channels at one stride, without a copy where the leading
+// dimensions collapse (contiguous tensors, channel slices of a packed projection).
+at::Tensor as_rows(const at::Tensor& x, int64_t* rows, int64_t* stride) {
+    const int64_t d = x.size(-1);
+    *rows = 1;
+    for (int64_t i = 0; i + 1 < x.dim(); ++i) *rows *= x.size(i);
+    int64_t step = -1, expect = -1;
+    bool ok = x.stride(-1) == 1 || d == 1;
+    for (int64_t i = x.dim() - 2; i >= 0 && ok; --i) {
+        if (x.size(i) == 1) continue;
+        if (step < 0) step = x.stride(i);
+        else ok = x.stride(i) == expect;
+        expect = x.stride(i) * x.size(i);
+    }
+    if (!ok) {
+        *stride = d;
+        return x.contiguous();
+    }
+    *stride = step < 0 ? d : step;
+    return x;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_cuda(const at::Tensor& x, const c10::optional<at::Tensor>& weight,
+                                                                 const c10::optional<at::Tensor>& residual, double eps,
+                                                                 bool quant, bool quant_only) {
+    TORCH_CHECK(x.is_cuda() && x.dim() >= 1 && x.size(-1) > 0, "add_rms_norm: x must be a CUDA tensor [..., D]");
+    const int64_t d = x.size(-1);
+    TORCH_CHECK(d <= std::numeric_limits<int32_t>::max(), "add_rms_norm: D is too large");
+    mindiesd_norm_args a = {};
+    at::Tensor xr = as_rows(x, &a.rows, &a.x_stride);
+    at::Tensor rr, wr, residual_out, scales;
+    at::Tensor out = at::empty(x.sizes(), x.options().dtype(quant ? at::kFloat8_e4m3fn : x.scalar_type()));
+    a.dtype = a.residual_dtype = a.weight_dtype = dtype_code(x.scalar_type());
+    a.dim = static_cast<int32_t>(d);
+    if (weight.has_value()) {
+        wr = weight.value().contiguous();
+        TORCH_CHECK(wr.is_cuda() && wr.device() == x.device() && wr.dim() == 1 && wr.size(0) == d,
+                    "add_rms_norm: weight must be a tensor [D] on the device of x");
+        a.weight = wr.data_ptr();
+        a.weight_dtype = dtype_code(wr.scalar_type());
+    }
+    if (residual.has_value()) {
+        const at::Tensor& r = residual.value();
+        TORCH_CHECK(r.is_cuda() && r.device() == x.device() && r.sizes() == x.sizes(),
+                    "add_rms_norm: residual must have the shape and the device of x");
+        int64_t rows = 0;
+        rr = as_rows(r, &rows, &a.residual_stride);
+        residual_out = at::empty(r.sizes(), r.options());
+        a.residual = rr.data_ptr();
+        a.residual_out = residual_out.data_ptr();
+        a.residual_dtype = dtype_code(r.scalar_type());
+    } else {
+        residual_out = at::empty({0}, x.options());
+    }
+    if (quant) {
+        std::vector<int64_t> shape = x.sizes().vec();
+        shape.back() = 1;
+        scales = at::empty(shape, x.options().dtype(at::kFloat));
+        a.scales = scales.data_ptr<float>();
+    } else {
+        scales = at::empty({0}, x.options().dtype(at::kFloat));
+    }
+    if (a.rows == 0) return std::make_tuple(out, scales, residual_out);
+    a.x = xr.data_ptr();
+    a.out = out.data_ptr();
+    a.out_dtype = quant ? MINDIESD_E4M3 : a.dtype;
+    a.quant_only = quant_only ? 1 : 0;
+    a.eps = static_cast<float>(eps);
+    c10::cuda::CUDAGuard guard(x.device());
+    check_rc(mindiesd_add_rms_norm(&a, stream_of(x)), "mindiesd_add_rms_norm");
+    return std::make_tuple(out, scales, residual_out);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(mindiesd, m) {
@@ -864,6 +938,9 @@ TORCH_LIBRARY(mindiesd, m) {
     m.def(
         "fp8_attention(Tensor query, Tensor key, Tensor value, Tensor q_scale, Tensor k_scale, Tensor v_scale, "
         "float scale, int k_block, int v_block, ScalarType out_dtype) -> Tensor");
+    m.def(
+        "add_rms_norm(Tensor x, Tensor? weight, Tensor? residual, float eps, bool quant, bool quant_only) "
+        "-> (Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(mindiesd, CUDA, m) {
@@ -883,4 +960,5 @@ TORCH_LIBRARY_IMPL(mindiesd, CUDA, m) {
     m.impl("fa_block_quant", &fa_block_quant_cuda);
     m.impl("fa_rotate_quant", &fa_rotate_quant_cuda);
     m.impl("fp8_attention", &fp8_attention_cuda);
+    m.impl("add_rms_norm", &add_rms_norm_cuda);
 }

@@ -143,6 +143,16 @@ class EstimateArgs(C.Structure):
     ]
 
 
+class NormArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("residual", C.c_void_p), ("weight", C.c_void_p),
+        ("out", C.c_void_p), ("residual_out", C.c_void_p), ("scales", C.c_void_p),
+        ("rows", C.c_int64), ("x_stride", C.c_int64), ("residual_stride", C.c_int64),
+        ("dim", C.c_int32), ("dtype", C.c_int32), ("residual_dtype", C.c_int32), ("weight_dtype", C.c_int32),
+        ("out_dtype", C.c_int32), ("quant_only", C.c_int32), ("eps", C.c_float),
+    ]
+
+
 MAX_RANKS = 8
 
 
@@ -194,7 +204,7 @@ def lib():
         for name in ("mindiesd_attention_fwd", "mindiesd_rf_rearrange", "mindiesd_rf_block_mask",
                      "mindiesd_rf_pool", "mindiesd_rf_mask_from_pooled", "mindiesd_fa_block_quant",
                      "mindiesd_sparse_block_estimate", "mindiesd_fa_rotate_quant", "mindiesd_rope",
-                     "mindiesd_ulysses_move"):
+                     "mindiesd_ulysses_move", "mindiesd_add_rms_norm"):
             fn = getattr(handle, name, None)
             if fn is not None:
                 fn.restype = C.c_int

@@ -1,5 +1,6 @@
 from .flash_attn import attention_forward, attention_forward_varlen, attention_forward_host, sparse_attention
+from .norm import add_rms_norm, add_rms_norm_quant
 from .rope import rotary_position_embedding
 
 __all__ = ["attention_forward", "attention_forward_varlen", "attention_forward_host", "sparse_attention",
-           "rotary_position_embedding"]
+           "add_rms_norm", "add_rms_norm_quant", "rotary_position_embedding"]

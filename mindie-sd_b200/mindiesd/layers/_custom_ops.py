@@ -211,3 +211,10 @@ def _fa_rotate_quant_fake(x, rot, block_size, head_first):
 @register_ops.register_mindie_fake_op("fp8_attention")
 def _fp8_attention_fake(query, key, value, q_scale, k_scale, v_scale, scale, k_block, v_block, out_dtype):
     return query.new_empty(query.shape, dtype=out_dtype)
+
+
+@register_ops.register_mindie_fake_op("add_rms_norm")
+def _add_rms_norm_fake(x, weight, residual, eps, quant, quant_only):
+    out = x.new_empty(x.shape, dtype=torch.float8_e4m3fn if quant else x.dtype)
+    scales = x.new_empty([*x.shape[:-1], 1] if quant else [0], dtype=torch.float32)
+    return out, scales, x.new_empty([0]) if residual is None else residual.new_empty(residual.shape)

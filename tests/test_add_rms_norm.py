@@ -1,0 +1,256 @@
+"""Residual addition + RMS norm, its e4m3 form and the per-token quantiser: refusals on the host, values on
+a GPU against the 64-bit formula.
+
+Tolerances: the last rounding is off by at most half a step of the output's type relative to the value
+(half a subnormal step below its normal range).  The fp32 arithmetic before it: a thread adds at most 48
+squares, then at most 10 + 32 partial sums (rows beyond 49152 channels: one addition per 1024 channels
+more), all positive, so the sum is off by less than 128 roundings of 2^-24, its root by half of that;
+with the root's own 2 ulp, the addition, three products and a division: less than 2^-17 in all."""
+import ctypes
+
+import pytest
+import torch
+
+from oracle import block_linear as ob
+
+F32_SLACK = 2.0 ** -17
+
+
+def _close(got, want, dtype):
+    want = want.double()
+    tol = want.abs() * (ob.half_step(dtype) + F32_SLACK) + ob.smallest_half_step(dtype)
+    worst = ((got.double() - want).abs() - tol).max().item()
+    assert worst <= 0, worst
+
+
+def _close_quant(q, scale, y):
+    want = ob.token_scale(y)
+    assert ((scale.double() - want).abs() <= want * F32_SLACK).all()
+    stored = q.double()
+    ideal = y / scale.double()
+    # e4m3: half a step of 2^-4 relative, 2^-10 below its normal range; the quotient itself is off by F32_SLACK
+    tol = ideal.abs() * (2.0 ** -4 + F32_SLACK) + 2.0 ** -10
+    assert ((stored - ideal).abs() <= tol).all()
+    assert stored.abs().max() <= 448
+
+
+def _randn(seed, *shape, dtype=torch.float32, scale=1.0, device="cuda"):
+    g = torch.Generator(device=device).manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device=device) * scale).to(dtype)
+
+
+# ---- host ------------------------------------------------------------------------------------------
+
+def test_struct_layout_and_codes_without_a_gpu(tmp_path):
+    import shutil
+    import subprocess
+    from pathlib import Path
+    from mindiesd import _cabi
+    lib = _cabi.lib()
+    a = _cabi.NormArgs()
+    fn = lib.mindiesd_add_rms_norm
+    assert fn(None, None) == -1 and fn(ctypes.byref(a), None) == -1
+    a.x = a.out = 4096
+    assert fn(ctypes.byref(a), None) == -2  # no rows
+    a.rows, a.dim, a.dtype, a.out_dtype, a.eps = 4, 64, 7, 0, 1e-6
+    assert fn(ctypes.byref(a), None) == -3
+    a.dtype = _cabi.BF16
+    a.out_dtype = _cabi.FP16
+    assert fn(ctypes.byref(a), None) == -3  # the output has the type of x, or is e4m3
+    a.out_dtype = _cabi.E4M3
+    assert fn(ctypes.byref(a), None) == -1  # e4m3 without scales
+    a.out_dtype, a.eps = _cabi.BF16, 0.0
+    assert fn(ctypes.byref(a), None) == -5
+    a.eps = 1e-6
+    a.residual = 4096
+    assert fn(ctypes.byref(a), None) == -1  # a residual without a place for the sum
+    a.residual_out, a.residual_dtype = 4096, _cabi.FP16
+    assert fn(ctypes.byref(a), None) == -3
+    a.residual_dtype, a.residual_stride = _cabi.BF16, -64
+    assert fn(ctypes.byref(a), None) == -4
+    a.residual_stride, a.x = 64, 4097
+    assert fn(ctypes.byref(a), None) == -4
+    a.x, a.quant_only = 4096, 1
+    assert fn(ctypes.byref(a), None) == -5  # the quantiser alone takes neither weight nor residual
+    cc = shutil.which("gcc")
+    if cc:
+        src = tmp_path / "s.c"
+        src.write_text('#include <stdio.h>\n#include "mindiesd_b200.h"\nint main(void){printf("%zu",sizeof(mindiesd_norm_args));return 0;}\n')
+        inc = Path(__file__).resolve().parent.parent / "include"
+        subprocess.run([cc, "-I", str(inc), str(src), "-o", str(tmp_path / "s")], check=True)
+        assert int(subprocess.run([str(tmp_path / "s")], capture_output=True, text=True, check=True).stdout) == \
+            ctypes.sizeof(_cabi.NormArgs)
+
+
+def test_refusals():
+    from mindiesd import ParametersInvalid, add_rms_norm, add_rms_norm_quant
+    from mindiesd.layers.quant import token_quant_preprocess
+    x = torch.zeros(4, 64, dtype=torch.bfloat16, device="meta")
+    bad = [
+        dict(x=[1.0]), dict(x=x.double()), dict(x=torch.zeros(4, 0, dtype=torch.bfloat16, device="meta")),
+        dict(x=torch.zeros(4, 64)),  # not on a CUDA device
+        dict(x=x, weight=torch.zeros(63, device="meta")), dict(x=x, weight=torch.zeros(64, dtype=torch.float16, device="meta")),
+        dict(x=x, weight=torch.zeros(64)), dict(x=x, weight=3.0),
+        dict(x=x, residual=x[:3]), dict(x=x, residual=x.half()), dict(x=x, residual=torch.zeros(4, 64)), dict(x=x, residual=0),
+        dict(x=x, eps=0.0), dict(x=x, eps=-1e-6), dict(x=x, eps=1), dict(x=x, eps=float("nan")),
+        dict(x=x, weight=torch.zeros(64, device="meta", requires_grad=True)),
+    ]
+    for kw in bad:
+        for fn in (add_rms_norm, add_rms_norm_quant):
+            with pytest.raises(ParametersInvalid):
+                fn(**kw)
+    for t in ([1.0], torch.zeros(4, 64), x.double(), torch.zeros((), device="meta"), x.float().requires_grad_()):
+        with pytest.raises(ParametersInvalid):
+            token_quant_preprocess(t)
+
+
+def test_fake_shapes():
+    from mindiesd import add_rms_norm, add_rms_norm_quant
+    from mindiesd.layers.quant import token_quant_preprocess
+    x = torch.zeros(2, 5, 64, dtype=torch.float16, device="meta")
+    r = torch.zeros(2, 5, 64, device="meta")
+    y, total = add_rms_norm(x, None, r)
+    assert y.dtype == torch.float16 and y.shape == x.shape and total.dtype == torch.float32 and total.shape == r.shape
+    q, s = add_rms_norm_quant(x)
+    assert q.dtype == torch.float8_e4m3fn and q.shape == x.shape and s.shape == (2, 5, 1) and s.dtype == torch.float32
+    q, s = token_quant_preprocess(x)
+    assert q.shape == x.shape and s.shape == (2, 5, 1)
+
+
+# ---- GPU -------------------------------------------------------------------------------------------
+
+DIMS = [1, 3, 8, 31, 64, 100, 128, 1001, 1004, 1536, 5120, 6143, 8192, 20480]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", DIMS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_values(dim, dtype):
+    from mindiesd import add_rms_norm, add_rms_norm_quant
+    for rows, weight, residual in [(1, None, None), (7, dtype, dtype), (33, torch.float32, torch.float32), (260, dtype, None)]:
+        x = _randn(dim + rows, rows, dim, dtype=dtype)
+        w = None if weight is None else _randn(1, dim, dtype=weight)
+        r = None if residual is None else _randn(2, rows, dim, dtype=residual, scale=3.0)
+        y64, v64 = ob.rms_norm(x, w, r)
+        got = add_rms_norm(x, w, r)
+        quant = add_rms_norm_quant(x, w, r)
+        if r is not None:
+            got, total = got
+            assert total.dtype == residual and torch.equal(quant[2], total)
+            _close(total, v64, residual)
+        assert got.dtype == dtype and got.shape == x.shape
+        _close(got, y64, dtype)
+        _close_quant(quant[0], quant[1], y64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("dim", [1, 65, 72, 1536, 5120])
+def test_token_quant(dim, dtype):
+    from mindiesd.layers.quant import token_quant_preprocess
+    x = _randn(dim, 2, 19, dim, dtype=dtype)
+    x[0, 3] = 0
+    x[1, 4] *= 1e-4
+    q, s = token_quant_preprocess(x)
+    assert s.shape == (2, 19, 1) and s[0, 3].item() == 1.0 and torch.count_nonzero(q[0, 3].float()) == 0
+    _close_quant(q, s, x.double())
+
+
+@pytest.mark.gpu
+def test_long_rows():
+    from mindiesd import add_rms_norm, add_rms_norm_quant
+    for dim, dtype in ((70001, torch.bfloat16), (70000, torch.float32), (6145, torch.float16)):
+        x, r = _randn(3, 5, dim, dtype=dtype), _randn(4, 5, dim, dtype=dtype)
+        w = _randn(5, dim)
+        y64, v64 = ob.rms_norm(x, w, r)
+        y, total = add_rms_norm(x, w, r)
+        _close(y, y64, dtype)
+        _close(total, v64, dtype)
+        q, s, _ = add_rms_norm_quant(x, w, r)
+        _close_quant(q, s, y64)
+
+
+@pytest.mark.gpu
+def test_strided_rows_and_empty_inputs():
+    from mindiesd import add_rms_norm, add_rms_norm_quant
+    from mindiesd.layers.quant import token_quant_preprocess
+    packed = _randn(7, 3, 50, 3 * 384, dtype=torch.bfloat16)
+    for part in (packed[..., :384], packed[..., 384:768], packed[..., 5:389], packed[:, ::2, :384], packed.transpose(0, 1)[..., 384:],
+                 packed[..., ::3], packed[:1].expand(3, 50, 1152)):
+        r = _randn(8, *part.shape, dtype=torch.bfloat16)
+        y, total = add_rms_norm(part, None, r)
+        y64, v64 = ob.rms_norm(part, None, r)
+        _close(y, y64, torch.bfloat16)
+        _close(total, v64, torch.bfloat16)
+        y2, total2 = add_rms_norm(r, None, part)
+        assert torch.equal(y2, y) and torch.equal(total2, total)  # a sum does not depend on the order of two terms
+    one = _randn(9, 384, dtype=torch.float16)
+    _close(add_rms_norm(one), ob.rms_norm(one)[0], torch.float16)
+    empty = torch.empty(0, 384, dtype=torch.bfloat16, device="cuda")
+    assert add_rms_norm(empty).shape == (0, 384)
+    q, s, t = add_rms_norm_quant(empty, None, empty)
+    assert q.shape == (0, 384) and s.shape == (0, 1) and t.shape == (0, 384)
+    assert token_quant_preprocess(empty)[1].shape == (0, 1)
+
+
+@pytest.mark.gpu
+def test_unusual_values():
+    """A row of zeros, one of the type's largest and smallest values, and rows with a NaN or an infinity stay apart."""
+    from mindiesd import add_rms_norm, add_rms_norm_quant
+    from mindiesd.layers.quant import token_quant_preprocess
+    for dim in (128, 129):
+        x = _randn(11, 8, dim, dtype=torch.bfloat16)
+        x[1] = 0
+        x[2, 5] = float("nan")
+        x[4, 7] = float("inf")
+        x[6] *= 1e-30
+        keep = [0, 1, 3, 5, 6, 7]
+        y = add_rms_norm(x)
+        q, s = add_rms_norm_quant(x)
+        y64 = ob.rms_norm(x)[0]
+        _close(y[keep], y64[keep], torch.bfloat16)
+        _close_quant(q[keep], s[keep], y64[keep])
+        assert s[1].item() == 1.0 and torch.isnan(s[2]) and torch.isnan(s[4])
+        assert torch.isnan(y[2].float()).all() and torch.isnan(y[4, 7]) and torch.isnan(q[2].float()).all()
+        tiny = torch.full((2, dim), 1e-40, device="cuda")
+        tiny[1] = torch.finfo(torch.float32).max
+        q, s = token_quant_preprocess(tiny)
+        _close_quant(q, s, tiny.double())
+        assert s[0].item() == 2.0 ** -126 and (q[1].float() == 448).all()
+        q, s = token_quant_preprocess(x)
+        assert torch.isnan(s[2]) and torch.isinf(s[4]) and torch.isfinite(s[keep]).all()
+
+
+@pytest.mark.gpu
+def test_many_short_rows_and_rows_beyond_32_bit_offsets():
+    from mindiesd import add_rms_norm, add_rms_norm_quant
+    x = _randn(12, 70001, 128, dtype=torch.float16)
+    w = _randn(13, 128, dtype=torch.float16)
+    _close(add_rms_norm(x, w), ob.rms_norm(x, w)[0], torch.float16)
+    x = torch.zeros(270000, 8192, dtype=torch.bfloat16, device="cuda")  # 2.2e9 elements
+    x[-3:] = _randn(14, 3, 8192, dtype=torch.bfloat16)
+    q, s = add_rms_norm_quant(x)
+    _close_quant(q[-3:], s[-3:], ob.rms_norm(x[-3:])[0])
+    assert s[-4].item() == 1.0
+
+
+@pytest.mark.gpu
+def test_streams_graphs_and_repeatability():
+    from mindiesd import add_rms_norm_quant
+    x, r = _randn(15, 300, 1536, dtype=torch.bfloat16), _randn(16, 300, 1536)
+    first = add_rms_norm_quant(x, None, r)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = add_rms_norm_quant(x, None, r)
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(first, second):
+        assert torch.equal(a.float(), b.float())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = add_rms_norm_quant(x, None, r)
+    x.copy_(_randn(17, 300, 1536, dtype=torch.bfloat16))
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(captured, add_rms_norm_quant(x, None, r)):
+        assert torch.equal(a.float(), b.float())
