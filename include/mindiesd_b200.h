@@ -474,6 +474,60 @@ typedef struct mindiesd_norm_args {
 int mindiesd_add_rms_norm(const mindiesd_norm_args* args, void* stream);
 
 /*
+ * Matrix product with its epilogue:
+ *   out = residual + gate * act(x weight^T * x_scale * weight_scale + bias)
+ * x: [m, k], weight: [n, k], both bf16, both fp16 or both e4m3 (in_dtype), k contiguous, rows x_stride /
+ * weight_stride elements apart (multiples of 16 bytes, 16-byte aligned; k itself may be any).  Products are
+ * accumulated in fp32, the epilogue runs in fp32, one rounding to out_dtype (bf16 or fp16).
+ * x_scale, weight_scale: e4m3 operands only (required then): fp32 [m] and [n], or one value each
+ * (x_scale_single / weight_scale_single).
+ * Each optional (NULL): bias [n]; residual [m, n] in out_dtype; gate [ceil(m / rows_per_gate), n], row i using
+ * gate row i / rows_per_gate (one gate per sample of a batch).  bias and gate are bf16, fp16 or fp32, each
+ * on its own.  out: rows out_stride elements apart; must not overlap an input.
+ * Any m, n, k >= 1.  The call allocates nothing and needs no workspace; results do not depend on timing.
+ *
+ * Stands in for the linear layers around attention that the reference leaves to torch (nn.Linear) and its
+ * dynamically quantised form (mindiesd/quantization/layer.py), with the activation of
+ * mindiesd/layers/activation.py and the gated residual addition of a modulated transformer block.
+ */
+enum {
+    MINDIESD_ACT_NONE = 0,
+    MINDIESD_ACT_RELU = 1,
+    MINDIESD_ACT_SILU = 2,
+    MINDIESD_ACT_GELU = 3,     /* v/2 (1 + erf(v / sqrt 2)) */
+    MINDIESD_ACT_GELU_TANH = 4 /* v/2 (1 + tanh(sqrt(2/pi) (v + 0.044715 v^3))) */
+};
+
+typedef struct mindiesd_linear_args {
+    const void* x;
+    const void* weight;
+    const void* bias;
+    const void* residual;
+    const void* gate;
+    const float* x_scale;
+    const float* weight_scale;
+    void* out;
+    int64_t x_stride; /* elements between rows */
+    int64_t weight_stride;
+    int64_t residual_stride;
+    int64_t gate_stride;
+    int64_t out_stride;
+    int32_t m, n, k;
+    int32_t rows_per_gate;
+    int32_t in_dtype;  /* MINDIESD_BF16 / FP16 / E4M3 */
+    int32_t out_dtype; /* MINDIESD_BF16 / FP16 */
+    int32_t bias_dtype;
+    int32_t gate_dtype;
+    int32_t x_scale_single;
+    int32_t weight_scale_single;
+    int32_t activation;
+    uint32_t wait_limit_us; /* as in mindiesd_attn_args: a wait that runs out leaves NaN and status 105 */
+    int32_t test_withhold;  /* test hook, 0 in production: the loaders withhold their copies */
+} mindiesd_linear_args;
+
+int mindiesd_linear_fwd(const mindiesd_linear_args* args, void* stream);
+
+/*
  * The re-shard step of Ulysses sequence parallelism as one data-movement kernel.
  *
  * A rank holds `rows` tokens with all N heads: tensors [rows, N, 128] addressed by a row and a head

@@ -881,6 +881,92 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_cuda(const at::Tenso
     return std::make_tuple(out, scales, residual_out);
 }
 
+// ---- matrix product with bias, activation, gate and residual ------------------------------------------------
+// Rows as the copy engine fetches them: 16-byte aligned, a multiple of 16 bytes apart, not overlapping.  Anything else
+// (an uneven width, a broadcast, an odd slice) is copied once to rows of a padded stride.
+at::Tensor as_tma_rows(const at::Tensor& x, int64_t* rows, int64_t* stride) {
+    at::Tensor r = as_rows(x, rows, stride);
+    const int64_t k = x.size(-1), e = x.element_size(), step = 16 / e;
+    if (*rows <= 1) *stride = (k + step - 1) / step * step;  // of no meaning for one row
+    if (reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 == 0 && *stride % step == 0 && *stride >= k) return r;
+    *stride = (k + step - 1) / step * step;
+    at::Tensor wide = at::empty({*rows, *stride}, x.options());
+    wide.narrow(1, 0, k).copy_(r.reshape({*rows, k}));
+    return wide;
+}
+
+at::Tensor linear_fwd_cuda(const at::Tensor& x, const at::Tensor& weight, const c10::optional<at::Tensor>& bias,
+                           const c10::optional<at::Tensor>& residual, const c10::optional<at::Tensor>& gate,
+                           const c10::optional<at::Tensor>& x_scale, const c10::optional<at::Tensor>& weight_scale,
+                           int64_t activation, at::ScalarType out_dtype) {
+    TORCH_CHECK(x.is_cuda() && weight.is_cuda() && x.device() == weight.device() && x.scalar_type() == weight.scalar_type(),
+                "linear_fwd: x and weight must be CUDA tensors of one device and one dtype");
+    TORCH_CHECK(x.dim() >= 1 && weight.dim() == 2 && x.size(-1) == weight.size(1) && weight.size(0) > 0 && weight.size(1) > 0,
+                "linear_fwd: x must be [..., K] and weight [N, K]");
+    const int64_t n = weight.size(0), k = weight.size(1), m = x.numel() / k;
+    constexpr int64_t kMost = std::numeric_limits<int32_t>::max();
+    TORCH_CHECK(m <= kMost && n <= kMost && k <= kMost, "linear_fwd: too many rows or columns");
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = n;
+    at::Tensor out = at::empty(shape, x.options().dtype(out_dtype));
+    mindiesd_linear_args a = {};
+    at::Tensor br, rr, gr, xsr, wsr;
+    auto on_device = [&](const at::Tensor& t) { return t.is_cuda() && t.device() == x.device(); };
+    if (bias.has_value()) {
+        br = bias.value().contiguous();
+        TORCH_CHECK(on_device(br) && br.dim() == 1 && br.size(0) == n, "linear_fwd: bias must be [N] on the device of x");
+        a.bias = br.data_ptr();
+        a.bias_dtype = dtype_code(br.scalar_type());
+    }
+    if (residual.has_value()) {
+        TORCH_CHECK(on_device(residual.value()) && residual.value().sizes() == out.sizes() && residual.value().scalar_type() == out_dtype,
+                    "linear_fwd: residual must have the shape, the dtype and the device of the output");
+        int64_t rows = 0;
+        rr = as_rows(residual.value(), &rows, &a.residual_stride);
+        a.residual = rr.data_ptr();
+    }
+    if (gate.has_value()) {
+        const at::Tensor& g = gate.value();
+        TORCH_CHECK(on_device(g) && g.dim() >= 1 && g.size(-1) == n, "linear_fwd: gate must be [N] or [B, 1, N] on the device of x");
+        int64_t rows = 0;
+        gr = as_rows(g, &rows, &a.gate_stride);
+        TORCH_CHECK(rows == 1 || (x.dim() >= 2 && rows == x.size(0)), "linear_fwd: one gate row, or one per entry of x's first dimension");
+        a.gate = gr.data_ptr();
+        a.gate_dtype = dtype_code(gr.scalar_type());
+        a.rows_per_gate = static_cast<int32_t>(rows > 0 && m > 0 ? m / rows : 1);
+    }
+    if (x_scale.has_value()) {
+        xsr = x_scale.value().contiguous();
+        TORCH_CHECK(on_device(xsr) && xsr.scalar_type() == at::kFloat && (xsr.numel() == m || xsr.numel() == 1),
+                    "linear_fwd: x_scale must be fp32, one value per row of x or one in all");
+        a.x_scale = xsr.data_ptr<float>();
+        a.x_scale_single = xsr.numel() == 1;
+    }
+    if (weight_scale.has_value()) {
+        wsr = weight_scale.value().contiguous();
+        TORCH_CHECK(on_device(wsr) && wsr.scalar_type() == at::kFloat && (wsr.numel() == n || wsr.numel() == 1),
+                    "linear_fwd: weight_scale must be fp32, one value per row of weight or one in all");
+        a.weight_scale = wsr.data_ptr<float>();
+        a.weight_scale_single = wsr.numel() == 1;
+    }
+    if (m == 0) return out;
+    c10::cuda::CUDAGuard guard(x.device());
+    int64_t rows_x = 0, rows_w = 0;
+    at::Tensor xr = as_tma_rows(x, &rows_x, &a.x_stride), wr = as_tma_rows(weight, &rows_w, &a.weight_stride);
+    a.x = xr.data_ptr();
+    a.weight = wr.data_ptr();
+    a.out = out.data_ptr();
+    a.out_stride = n;
+    a.m = static_cast<int32_t>(m);
+    a.n = static_cast<int32_t>(n);
+    a.k = static_cast<int32_t>(k);
+    a.in_dtype = dtype_code(x.scalar_type());
+    a.out_dtype = dtype_code(out_dtype);
+    a.activation = static_cast<int32_t>(activation);
+    check_rc(mindiesd_linear_fwd(&a, stream_of(x)), "mindiesd_linear_fwd");
+    return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(mindiesd, m) {
@@ -941,6 +1027,9 @@ TORCH_LIBRARY(mindiesd, m) {
     m.def(
         "add_rms_norm(Tensor x, Tensor? weight, Tensor? residual, float eps, bool quant, bool quant_only) "
         "-> (Tensor, Tensor, Tensor)");
+    m.def(
+        "linear_fwd(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, Tensor? gate, Tensor? x_scale, "
+        "Tensor? weight_scale, int activation, ScalarType out_dtype) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(mindiesd, CUDA, m) {
@@ -961,4 +1050,5 @@ TORCH_LIBRARY_IMPL(mindiesd, CUDA, m) {
     m.impl("fa_rotate_quant", &fa_rotate_quant_cuda);
     m.impl("fp8_attention", &fp8_attention_cuda);
     m.impl("add_rms_norm", &add_rms_norm_cuda);
+    m.impl("linear_fwd", &linear_fwd_cuda);
 }

@@ -153,6 +153,21 @@ class NormArgs(C.Structure):
     ]
 
 
+class LinearArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p), ("residual", C.c_void_p), ("gate", C.c_void_p),
+        ("x_scale", C.c_void_p), ("weight_scale", C.c_void_p), ("out", C.c_void_p),
+        ("x_stride", C.c_int64), ("weight_stride", C.c_int64), ("residual_stride", C.c_int64),
+        ("gate_stride", C.c_int64), ("out_stride", C.c_int64),
+        ("m", C.c_int32), ("n", C.c_int32), ("k", C.c_int32), ("rows_per_gate", C.c_int32),
+        ("in_dtype", C.c_int32), ("out_dtype", C.c_int32), ("bias_dtype", C.c_int32), ("gate_dtype", C.c_int32),
+        ("x_scale_single", C.c_int32), ("weight_scale_single", C.c_int32), ("activation", C.c_int32),
+        ("wait_limit_us", C.c_uint32), ("test_withhold", C.c_int32),
+    ]
+
+
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+
 MAX_RANKS = 8
 
 
@@ -204,7 +219,7 @@ def lib():
         for name in ("mindiesd_attention_fwd", "mindiesd_rf_rearrange", "mindiesd_rf_block_mask",
                      "mindiesd_rf_pool", "mindiesd_rf_mask_from_pooled", "mindiesd_fa_block_quant",
                      "mindiesd_sparse_block_estimate", "mindiesd_fa_rotate_quant", "mindiesd_rope",
-                     "mindiesd_ulysses_move", "mindiesd_add_rms_norm"):
+                     "mindiesd_ulysses_move", "mindiesd_add_rms_norm", "mindiesd_linear_fwd"):
             fn = getattr(handle, name, None)
             if fn is not None:
                 fn.restype = C.c_int

@@ -218,3 +218,8 @@ def _add_rms_norm_fake(x, weight, residual, eps, quant, quant_only):
     out = x.new_empty(x.shape, dtype=torch.float8_e4m3fn if quant else x.dtype)
     scales = x.new_empty([*x.shape[:-1], 1] if quant else [0], dtype=torch.float32)
     return out, scales, x.new_empty([0]) if residual is None else residual.new_empty(residual.shape)
+
+
+@register_ops.register_mindie_fake_op("linear_fwd")
+def _linear_fwd_fake(x, weight, bias, residual, gate, x_scale, weight_scale, activation, out_dtype):
+    return x.new_empty([*x.shape[:-1], weight.shape[0]], dtype=out_dtype)

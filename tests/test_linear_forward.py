@@ -1,0 +1,273 @@
+"""`linear_forward`: refusals on the host, values on a GPU against the 64-bit formula.
+
+Tolerances: one last rounding (half a step relative to the value), plus the fp32 accumulation: products of two-byte
+or e4m3 values are exact in fp32, a tensor-core instruction adds at least 8 of them to a running sum that may be
+truncated, so each step is off by at most 2^-23 of the largest partial sum, which the sum of |x||w| bounds:
+(K/8 + 8) 2^-23 sum|x||w| (carried through the epilogue by the oracle).  The activations' own error is below 2^-15
+relative: their exponent's argument is rounded to fp32 (|v| < 90 times 2^-24 times log2 e) and erfc amplifies its
+argument's rounding by v^2."""
+import ctypes
+
+import pytest
+import torch
+
+from oracle import block_linear as ob
+
+ACT_SLACK = 2.0 ** -15
+
+
+def _randn(seed, *shape, dtype=torch.float32, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def _operands(seed, m, k, n, dtype):
+    """(x, weight, keyword arguments): e4m3 operands come with their scales."""
+    if dtype != torch.float8_e4m3fn:
+        return _randn(seed, m, k, dtype=dtype), _randn(seed + 1, n, k, dtype=dtype, scale=k ** -0.5), {}
+    from mindiesd.layers.quant import token_quant_preprocess
+    x, xs = token_quant_preprocess(_randn(seed, m, k))
+    w, ws = token_quant_preprocess(_randn(seed + 1, n, k, scale=k ** -0.5))
+    return x, w, dict(x_scale=xs, weight_scale=ws)
+
+
+def _check(got, x, w, out_dtype, k, **kw):
+    want, size = ob.linear(x, w, **kw)
+    assert got.dtype == out_dtype and got.shape == want.shape
+    tol = want.abs() * (ob.half_step(out_dtype) + ACT_SLACK) + ob.smallest_half_step(out_dtype) + size * (k / 8 + 8) * 2.0 ** -23
+    worst = ((got.double() - want).abs() - tol).max().item()
+    assert worst <= 0, worst
+
+
+# ---- host ------------------------------------------------------------------------------------------
+
+def test_codes_without_a_gpu(tmp_path):
+    import shutil
+    import subprocess
+    from pathlib import Path
+    from mindiesd import _cabi
+    fn = _cabi.lib().mindiesd_linear_fwd
+    a = _cabi.LinearArgs()
+    assert fn(None, None) == -1 and fn(ctypes.byref(a), None) == -1
+    a.x = a.weight = a.out = 4096
+    assert fn(ctypes.byref(a), None) == -2
+    a.m, a.n, a.k = 4, 64, 64
+    a.x_stride = a.weight_stride = a.out_stride = 64
+    for field, value, code in [("in_dtype", _cabi.FP32, -3), ("out_dtype", _cabi.FP32, -3), ("in_dtype", _cabi.E4M3, -1),
+                               ("x_scale", 4096, -5), ("activation", 5, -5), ("activation", -1, -5), ("x_stride", 0, -4),
+                               ("x_stride", 63, -4), ("weight_stride", 0, -4), ("out_stride", 32, -4), ("out", 4097, -4),
+                               ("m", 0x7fffffff, -7), ("n", 0, -2), ("k", -1, -2)]:
+        b = _cabi.LinearArgs.from_buffer_copy(a)
+        setattr(b, field, value)
+        assert fn(ctypes.byref(b), None) == code, (field, value)
+    b = _cabi.LinearArgs.from_buffer_copy(a)
+    b.bias, b.bias_dtype = 4096, _cabi.E4M3
+    assert fn(ctypes.byref(b), None) == -3
+    b.bias, b.bias_dtype = 4098, _cabi.FP32
+    assert fn(ctypes.byref(b), None) == -4
+    b = _cabi.LinearArgs.from_buffer_copy(a)
+    b.gate = 4096
+    assert fn(ctypes.byref(b), None) == -5  # no rows per gate
+    b.rows_per_gate, b.gate_stride = 4, -64
+    assert fn(ctypes.byref(b), None) == -4
+    cc = shutil.which("gcc")
+    if cc:
+        src = tmp_path / "s.c"
+        src.write_text('#include <stdio.h>\n#include "mindiesd_b200.h"\nint main(void){printf("%zu",sizeof(mindiesd_linear_args));return 0;}\n')
+        inc = Path(__file__).resolve().parent.parent / "include"
+        subprocess.run([cc, "-I", str(inc), str(src), "-o", str(tmp_path / "s")], check=True)
+        assert int(subprocess.run([str(tmp_path / "s")], capture_output=True, text=True, check=True).stdout) == \
+            ctypes.sizeof(_cabi.LinearArgs)
+
+
+def test_refusals():
+    from mindiesd import ParametersInvalid, linear_forward
+
+    def t(*shape, dtype=torch.bfloat16):
+        return torch.zeros(shape, dtype=dtype, device="meta")
+    x, w = t(2, 5, 64), t(32, 64)
+    x8, w8 = t(2, 5, 64, dtype=torch.float8_e4m3fn), t(32, 64, dtype=torch.float8_e4m3fn)
+    s, ws = t(2, 5, 1, dtype=torch.float32), t(32, dtype=torch.float32)
+    bad = [
+        dict(x=[1.0], weight=w), dict(x=x, weight=None), dict(x=x, weight=t(32, 63)), dict(x=x, weight=t(32, 64, 1)),
+        dict(x=x, weight=t(0, 64)), dict(x=t(5, 0), weight=t(32, 0)), dict(x=t(), weight=w), dict(x=x.float(), weight=w.float()),
+        dict(x=x, weight=w.half()), dict(x=x, weight=torch.zeros(32, 64, dtype=torch.bfloat16)),
+        dict(x=torch.zeros(5, 64, dtype=torch.bfloat16), weight=torch.zeros(32, 64, dtype=torch.bfloat16)),
+        dict(x=x, weight=w, activation="swish"), dict(x=x, weight=w, activation=None), dict(x=x, weight=w, out_dtype=torch.float32),
+        dict(x=x, weight=w, bias=t(33)), dict(x=x, weight=w, bias=t(1, 32)), dict(x=x, weight=w, bias=t(32, dtype=torch.float64)),
+        dict(x=x, weight=w, bias=torch.zeros(32)), dict(x=x, weight=w, bias=0.0),
+        dict(x=x, weight=w, residual=t(2, 5, 33)), dict(x=x, weight=w, residual=t(10, 32)), dict(x=x, weight=w, residual=t(2, 5, 32).half()),
+        dict(x=x, weight=w, gate=t(31)), dict(x=x, weight=w, gate=t(3, 1, 32)), dict(x=x, weight=w, gate=t(2, 5, 32)),
+        dict(x=x, weight=w, gate=t(5, 32)), dict(x=x, weight=w, gate=t(32, dtype=torch.int32)), dict(x=t(64), weight=w, gate=t(2, 32)),
+        dict(x=x, weight=w, x_scale=s, weight_scale=ws), dict(x=x8, weight=w8), dict(x=x8, weight=w8, x_scale=s),
+        dict(x=x8, weight=w, x_scale=s, weight_scale=ws), dict(x=x8, weight=w8, x_scale=s.half(), weight_scale=ws),
+        dict(x=x8, weight=w8, x_scale=t(10, dtype=torch.float32), weight_scale=ws),
+        dict(x=x8, weight=w8, x_scale=s, weight_scale=t(31, dtype=torch.float32)),
+        dict(x=x8, weight=w8, x_scale=s, weight_scale=1.0),
+        dict(x=x, weight=torch.nn.Parameter(w)),
+    ]
+    for kw in bad:
+        with pytest.raises(ParametersInvalid):
+            linear_forward(**kw)
+    assert linear_forward(x, w).shape == (2, 5, 32) and linear_forward(x8, w8, x_scale=s, weight_scale=ws).dtype == torch.bfloat16
+    assert linear_forward(x8, w8, x_scale=s[..., 0], weight_scale=ws[:, None], residual=t(2, 5, 32).half()).dtype == torch.float16
+    with torch.no_grad():
+        assert linear_forward(t(64), torch.nn.Parameter(w)).shape == (32,)
+
+
+# ---- GPU -------------------------------------------------------------------------------------------
+
+SHAPES = [(1, 256, 5120), (2, 64, 16), (1, 1, 1), (3, 8, 130), (16, 1001, 129), (17, 200, 1000), (64, 1536, 1536), (100, 4096, 257),
+          (128, 72, 256), (129, 72, 256), (200, 520, 33), (256, 64, 256), (257, 1024, 1000), (300, 1536, 1001), (513, 5120, 640),
+          (1000, 333, 514), (2048, 128, 2048), (5000, 256, 96)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", SHAPES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float8_e4m3fn])
+def test_product(m, k, n, dtype):
+    from mindiesd import linear_forward
+    x, w, kw = _operands(m + k + n, m, k, n, dtype)
+    for out_dtype in (torch.bfloat16, torch.float16):
+        _check(linear_forward(x, w, out_dtype=out_dtype, **kw), x, w, out_dtype, k, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", [(2, 200, 264), (48, 136, 129), (258, 320, 200), (600, 64, 333)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "gelu_tanh"])
+def test_epilogue(m, k, n, dtype, act):
+    from mindiesd import linear_forward
+    x, w, kw = _operands(m, m, k, n, dtype)
+    for bias_dtype, gate_dtype, out_dtype in [(torch.bfloat16, torch.float32, torch.bfloat16), (torch.float32, torch.float16, torch.float16),
+                                              (None, torch.bfloat16, torch.bfloat16), (torch.float16, None, torch.float16)]:
+        full = dict(kw)
+        if bias_dtype is not None:
+            full["bias"] = _randn(5, n, dtype=bias_dtype, scale=2.0)
+        if gate_dtype is not None:
+            full["gate"] = _randn(6, n, dtype=gate_dtype)
+        full["residual"] = _randn(7, m, n, dtype=out_dtype)
+        got = linear_forward(x, w, activation=act, out_dtype=out_dtype, **full)
+        _check(got, x, w, out_dtype, k, act=act, **full)
+        del full["residual"]
+        got = linear_forward(x, w, activation=act, out_dtype=out_dtype, **full)
+        _check(got, x, w, out_dtype, k, act=act, **full)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,rows", [(2, 3), (3, 40), (2, 300), (5, 130), (7, 1)])
+def test_gate_per_sample(batch, rows):
+    from mindiesd import linear_forward
+    x, w, _ = _operands(9, batch * rows, 192, 136, torch.bfloat16)
+    x = x.view(batch, rows, 192)
+    gate, residual = _randn(10, batch, 1, 136), _randn(11, batch, rows, 136, dtype=torch.bfloat16)
+    got = linear_forward(x, w, gate=gate, residual=residual)
+    _check(got, x, w, torch.bfloat16, 192, gate=gate, residual=residual)
+    assert torch.equal(got, linear_forward(x, w, gate=gate[:, 0], residual=residual))
+    flat = linear_forward(x.reshape(-1, 192), w, gate=gate.expand(batch, rows, 136).reshape(-1, 136), residual=residual.reshape(-1, 136))
+    assert torch.equal(flat.view_as(got), got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [5, 300])
+def test_strides_and_alignment(m):
+    """Slices of packed projections, transposes, broadcast rows, odd starts: read in place or copied, same answer."""
+    from mindiesd import linear_forward
+    k, n = 128, 72
+    pool = _randn(20, m, 3 * k + 8, dtype=torch.float16)
+    wpool = _randn(21, n, 2 * k + 8, dtype=torch.float16, scale=0.1)
+    rpool = _randn(22, m, 2 * n + 1, dtype=torch.float16)
+    for x in (pool[:, k:2 * k], pool[:, 3:3 + k], pool[:, :3 * k:3], pool[:1, :k].expand(m, k), _randn(23, k, m, dtype=torch.float16).t()):
+        for w in (wpool[:, k:2 * k], wpool[:, 1:1 + k], wpool[:1, :k].expand(n, k)):
+            for r in (rpool[:, :n], rpool[:, n:2 * n], rpool[:, :2 * n:2], rpool[:1, :n].expand(m, n)):
+                _check(linear_forward(x, w, residual=r), x, w, torch.float16, k, residual=r)
+    bias = _randn(24, 2 * n + 1)
+    for b in (bias[1:1 + n], bias[:2 * n:2]):
+        _check(linear_forward(pool[:, :k], wpool[:, :k], b), pool[:, :k], wpool[:, :k], torch.float16, k, bias=b)
+
+
+@pytest.mark.gpu
+def test_single_scales_and_three_dimensions():
+    from mindiesd import linear_forward
+    for m in (6, 400):
+        x = _randn(30, 2, m // 2, 96).to(torch.float8_e4m3fn)
+        w = _randn(31, 40, 96).to(torch.float8_e4m3fn)
+        kw = dict(x_scale=torch.tensor([0.37], device="cuda"), weight_scale=torch.tensor(0.11, device="cuda"))
+        _check(linear_forward(x, w, **kw), x, w, torch.bfloat16, 96, **kw)
+    x, w, _ = _operands(32, 1, 96, 40, torch.bfloat16)
+    assert torch.equal(linear_forward(x[0], w), linear_forward(x, w)[0])
+    assert linear_forward(x[:0], w).shape == (0, 40)
+    assert linear_forward(x.view(1, 1, 96)[:, :0], w, gate=_randn(33, 40)).shape == (1, 0, 40)
+
+
+@pytest.mark.gpu
+def test_rows_do_not_depend_on_their_neighbours():
+    """A NaN or an infinity stays in its row (or in its column, when it is in the weights)."""
+    from mindiesd import linear_forward
+    for m in (9, 300):
+        x, w, _ = _operands(40, m, 320, 200, torch.bfloat16)
+        clean = linear_forward(x, w)
+        x2, w2 = x.clone(), w.clone()
+        x2[3, 17] = float("nan")
+        w2[11, 5] = float("inf")
+        got = linear_forward(x2, w2)
+        assert torch.isnan(got[3].float()).all() and not torch.isfinite(got[:, 11].float()).any()
+        keep = torch.ones_like(got, dtype=torch.bool)
+        keep[3] = False
+        keep[:, 11] = False
+        assert torch.equal(got[keep], clean[keep])
+
+
+@pytest.mark.gpu
+def test_repeatable_on_streams_and_in_graphs():
+    from mindiesd import linear_forward
+    for m in (4, 700):
+        x, w, _ = _operands(50, m, 4096, 384, torch.bfloat16)
+        first = linear_forward(x, w)
+        streams = [torch.cuda.Stream() for _ in range(3)]
+        outs = []
+        for s in streams:  # several calls at once, of both kernels: nothing is shared between them
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                outs += [linear_forward(x, w) for _ in range(4)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(first, o) for o in outs)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured = linear_forward(x, w)
+        x.copy_(_randn(51, m, 4096, dtype=torch.bfloat16))
+        graph.replay()
+        assert torch.equal(captured, linear_forward(x, w))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [4, 700])
+def test_withheld_copies_give_up_cleanly(m):
+    from mindiesd import _cabi, linear_forward
+    assert _cabi.device_status() == 0
+    x, w, _ = _operands(60, m, 1024, 2048, torch.bfloat16)
+    out = torch.zeros(m, 2048, dtype=torch.bfloat16, device="cuda")
+    a = _cabi.LinearArgs()
+    a.x, a.weight, a.out = x.data_ptr(), w.data_ptr(), out.data_ptr()
+    a.x_stride = a.weight_stride = 1024
+    a.out_stride, a.m, a.n, a.k = 2048, m, 2048, 1024
+    a.in_dtype = a.out_dtype = _cabi.BF16
+    a.wait_limit_us, a.test_withhold = 20000, 1
+    _cabi.check(_cabi.lib().mindiesd_linear_fwd(ctypes.byref(a), _cabi.current_stream_ptr(x.device)), "mindiesd_linear_fwd")
+    torch.cuda.synchronize()
+    assert torch.isnan(out.float()).all()
+    assert torch.isnan(linear_forward(x, w).float()).all()  # while the word is set, later launches mark their rows too
+    assert _cabi.device_status() == 105 and _cabi.device_status() == 0
+    _check(linear_forward(x, w), x, w, torch.bfloat16, 1024)
+    assert _cabi.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    from mindiesd import linear_forward
+    x = torch.zeros(1100000, 64, dtype=torch.bfloat16, device="cuda")
+    x[-2:] = _randn(70, 2, 64, dtype=torch.bfloat16)
+    w = _randn(71, 2048, 64, dtype=torch.bfloat16)
+    out = linear_forward(x, w)  # 2.25e9 elements
+    _check(out[-2:], x[-2:], w, torch.bfloat16, 64)
+    assert torch.count_nonzero(out[-300:-2]).item() == 0
