@@ -39,7 +39,7 @@ struct Epilogue {
     int x_scale_step, w_scale_step;  // 0: one scale for all
     int bias_type, gate_type;        // MINDIESD_BF16 / FP16 / FP32
     int out_fp16, act;
-    int wide_out, wide_residual, wide_cols;  // rows (column vectors) can be moved 16 bytes at a time
+    int wide_out, wide_residual, wide_gate;  // rows can be moved 16 bytes at a time
     int m, n;
 };
 
@@ -56,6 +56,8 @@ struct LinearParams {
     int test_withhold;
     int* status;
 };
+
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
 __device__ __forceinline__ float load_any(const void* p, int type, int64_t i) {
     if (type == MINDIESD_FP32) return __ldg(static_cast<const float*>(p) + i);
@@ -83,7 +85,17 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi, int fp16) {
     return *reinterpret_cast<const uint32_t*>(&b);
 }
 
-// Eight consecutive column values (bias, gate, weight scale); every lane of a warp reads the same ones.
+template <bool kFp16, int kPairs>
+__device__ __forceinline__ void pack_values(const uint64_t (&v)[kPairs], uint32_t (&w)[kPairs]) {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+        float lo, hi;
+        unpack2(v[i], lo, hi);
+        w[i] = pack_pair(lo, hi, kFp16);
+    }
+}
+
+// Eight consecutive column values of the gate row that starts at row_at.
 __device__ __forceinline__ void load_cols8(const void* p, int type, int64_t row_at, int col, int n, bool wide, float (&f)[8]) {
     if (wide && col + 8 <= n) {
         if (type == MINDIESD_FP32) {
@@ -104,32 +116,62 @@ __device__ __forceinline__ void load_cols8(const void* p, int type, int64_t row_
     }
 }
 
-// The activations in the forms that keep their relative accuracy for large negative arguments:
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint64_t both(float v) { return pack2(v, v); }
+
+// v / (1 + 2^x) for a pair; 2^x may be infinite (the quotient is then 0).
+__device__ __forceinline__ uint64_t over_one_plus_ex2(uint64_t v, uint64_t x) {
+    float lo, hi;
+    unpack2(x, lo, hi);
+    const uint64_t d = add2(pack2(ex2_approx(lo), ex2_approx(hi)), both(1.0f));
+    unpack2(d, lo, hi);
+    return mul2(v, pack2(rcp_approx(lo), rcp_approx(hi)));
+}
+
+// Out of line: 32 copies of erfc in the epilogue's loop cost registers that the other activations need.
+__device__ __noinline__ float gelu_erf(float v) { return 0.5f * v * erfcf(-0.70710678118654752f * v); }
+
+// The activations, on pairs of values, in the forms that keep their relative accuracy for large negative arguments:
 //   gelu(v) = v/2 erfc(-v / sqrt 2),  silu(v) = v / (1 + e^-v),
 //   gelu_tanh(v) = v/2 (1 + tanh u) = v / (1 + e^-2u),  u = sqrt(2/pi) (v + 0.044715 v^3).
-__device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.0f + __expf(-v)); }
-__device__ __forceinline__ float gelu_tanh(float v) {
-    const float u2 = v * fmaf(0.07135481627f, v * v, 1.595769122f);
-    return __fdividef(v, 1.0f + __expf(-u2));
-}
-template <int kN>
-__device__ __forceinline__ void activate(float (&v)[kN], int act) {
+template <int kPairs>
+__device__ __forceinline__ void activate(uint64_t (&v)[kPairs], int act) {
+    constexpr float kLog2e = 1.4426950408889634f;
+    constexpr float kU1 = -2.0f * 0.7978845608028654f * kLog2e, kU3 = kU1 * 0.044715f;
     switch (act) {
         case kRelu:
 #pragma unroll
-            for (int i = 0; i < kN; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];  // a NaN stays
+            for (int i = 0; i < kPairs; ++i) {
+                float lo, hi;
+                unpack2(v[i], lo, hi);
+                v[i] = pack2(lo < 0.0f ? 0.0f : lo, hi < 0.0f ? 0.0f : hi);  // a NaN stays
+            }
             break;
         case kSilu:
 #pragma unroll
-            for (int i = 0; i < kN; ++i) v[i] = silu(v[i]);
+            for (int i = 0; i < kPairs; ++i) v[i] = over_one_plus_ex2(v[i], mul2(v[i], both(-kLog2e)));
             break;
         case kGelu:
 #pragma unroll
-            for (int i = 0; i < kN; ++i) v[i] = 0.5f * v[i] * erfcf(-0.70710678118654752f * v[i]);
+            for (int i = 0; i < kPairs; ++i) {
+                float lo, hi;
+                unpack2(v[i], lo, hi);
+                v[i] = pack2(gelu_erf(lo), gelu_erf(hi));
+            }
             break;
         case kGeluTanh:
 #pragma unroll
-            for (int i = 0; i < kN; ++i) v[i] = gelu_tanh(v[i]);
+            for (int i = 0; i < kPairs; ++i)
+                v[i] = over_one_plus_ex2(v[i], mul2(v[i], fma2(mul2(v[i], v[i]), both(kU3), both(kU1))));
             break;
         default: break;
     }
@@ -146,56 +188,83 @@ __device__ __forceinline__ void report(const LinearParams& p, const volatile int
 
 // ---- many rows ---------------------------------------------------------------------------------------------
 
-constexpr int kPairThreads = 384;  // warps: 0 loader, 1 MMA, 2 tensor memory, 3 idle, 4..11 epilogue
-constexpr int kPairStages = 6;
-constexpr int kPairStageBytes = 2 * kRowTile;
-constexpr int kStagingBytes = 32 * 64;  // per epilogue warp: 32 rows of 32 two-byte values
-constexpr int kPairSmem = kPairStages * kPairStageBytes + 8 * kStagingBytes + 256 + 1024;
+constexpr int kEpilogueWarps = 16;
+constexpr int kPairThreads = 128 + 32 * kEpilogueWarps;  // warps: 0 loader, 1 MMA, 2 tensor memory, 3 idle, 4.. epilogue
+constexpr int kSub = 2;  // k steps per ring stage: one barrier round trip and one commit for eight MMAs
+constexpr int kPairStages = 6 / kSub;
+constexpr int kPairStepBytes = 2 * kRowTile;
+constexpr int kPairStageBytes = kSub * kPairStepBytes;
+// The epilogue works in units of 32 rows x 16 columns.  Four warps share a quarter of the tile's rows and take its
+// units in turn: with two warps of 32-column units a 256-column tile left 4 us of epilogue after its last MMA, and
+// the latency of one warp's instructions, not their number, was what it waited for.
+constexpr int kUnit = 16;
+constexpr int kUnitWarps = kEpilogueWarps / 4;
+constexpr int kMaxUnits = 256 / kUnit / kUnitWarps;  // of one warp in one tile
+constexpr int kStagingBytes = 32 * kUnit * 2;        // per warp: one unit of two-byte values
+constexpr int kColsBytes = 3 * kMaxUnits * kUnit * 4;  // per warp: bias, weight scale and gate of its columns as fp32
+constexpr int kPairSmem = kPairStages * kPairStageBytes + kEpilogueWarps * (kStagingBytes + kColsBytes) + 256 + 1024;
+static_assert(kPairSmem <= 227 * 1024, "shared memory of the pair kernel");
 
-// Offset of 16-byte chunk c of row r in a warp's staging buffer; the exclusive or keeps both the row-wise writes and
-// the chunk-wise reads free of bank conflicts.
-__device__ __forceinline__ uint32_t staged(int r, int c) { return r * 64 + ((c ^ ((r >> 1) & 3)) << 4); }
+// Offset of 16-byte piece c of row r in a warp's staging buffer; the exclusive or keeps both the row-wise writes and
+// the piece-wise reads free of bank conflicts.
+__device__ __forceinline__ uint32_t staged(int r, int c) { return r * 32 + ((c ^ ((r >> 2) & 1)) << 4); }
 
-// Moves the 32 x 32 block at (row0, col0) of a two-byte row-major matrix between global memory and the staging
-// buffer; lanes cover 8 rows of 64 bytes at a time, or one row of 32 elements where 16-byte access is not possible.
-__device__ __forceinline__ void stage_in(char* buf, const uint16_t* g, int64_t stride, int row0, int col0, int m, int n, bool wide,
-                                         int lane) {
-    if (wide) {
-        const int c = lane & 3;
+// A lane's share of a unit in a two-byte row-major matrix: 8 columns of rows lane/2 and lane/2 + 16 of the warp's 32.
+struct UnitAt {
+    const uint16_t* p[2];
+    bool live[2];  // the rows exist
+    __device__ __forceinline__ UnitAt(const void* base, int64_t stride, int row0, int m, int lane) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = i * 8 + (lane >> 2);
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (row0 + r < m && col0 + c * 8 < n)
-                v = __ldg(reinterpret_cast<const uint4*>(g + static_cast<int64_t>(row0 + r) * stride + col0 + c * 8));
-            *reinterpret_cast<uint4*>(buf + staged(r, c)) = v;
+        for (int i = 0; i < 2; ++i) {
+            const int r = row0 + i * 16 + (lane >> 1);
+            live[i] = r < m;
+            p[i] = static_cast<const uint16_t*>(base) + static_cast<int64_t>(r) * stride + (lane & 1) * 8;
         }
-    } else {
-#pragma unroll 4
-        for (int r = 0; r < 32; ++r) {
-            uint16_t v = 0;
-            if (row0 + r < m && col0 + lane < n) v = g[static_cast<int64_t>(row0 + r) * stride + col0 + lane];
-            *reinterpret_cast<uint16_t*>(buf + staged(r, lane >> 3) + (lane & 7) * 2) = v;
+    }
+};
+
+__device__ __forceinline__ void fetch_unit(uint4 (&v)[2], const UnitAt& at, int col0, int n, bool wide, int lane) {
+    const int left = n - col0 - (lane & 1) * 8;  // columns of this lane that exist
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        v[i] = make_uint4(0, 0, 0, 0);
+        if (!at.live[i] || left <= 0) continue;
+        if (wide) {
+            v[i] = __ldg(reinterpret_cast<const uint4*>(at.p[i] + col0));
+        } else {
+            uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j < left) w[j >> 1] |= static_cast<uint32_t>(at.p[i][col0 + j]) << ((j & 1) * 16);
+            v[i] = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
 }
-__device__ __forceinline__ void stage_out(const char* buf, uint16_t* g, int64_t stride, int row0, int col0, int m, int n, bool wide,
-                                          int lane) {
-    if (wide) {
-        const int c = lane & 3;
+__device__ __forceinline__ void put_unit(char* buf, const uint4 (&v)[2], int lane) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = i * 8 + (lane >> 2);
-            if (row0 + r < m && col0 + c * 8 < n)
-                *reinterpret_cast<uint4*>(g + static_cast<int64_t>(row0 + r) * stride + col0 + c * 8) =
-                    *reinterpret_cast<const uint4*>(buf + staged(r, c));
+    for (int i = 0; i < 2; ++i) *reinterpret_cast<uint4*>(buf + staged(i * 16 + (lane >> 1), lane & 1)) = v[i];
+}
+
+// Writes a warp's staging buffer to the output: 16 rows of 32 bytes at a time, or two rows of 16 elements where 16-byte
+// access is not possible.
+__device__ __forceinline__ void stage_out(const char* buf, const UnitAt& at, const Epilogue& e, int row0, int col0, int lane) {
+    if (e.wide_out) {
+        if (col0 + (lane & 1) * 8 < e.n) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (at.live[i])
+                    *reinterpret_cast<uint4*>(const_cast<uint16_t*>(at.p[i]) + col0) =
+                        *reinterpret_cast<const uint4*>(buf + staged(i * 16 + (lane >> 1), lane & 1));
         }
     } else {
+        const int c = lane & 15;
+        uint16_t* g = static_cast<uint16_t*>(e.out) + static_cast<int64_t>(row0) * e.out_stride + col0 + c;
 #pragma unroll 4
-        for (int r = 0; r < 32; ++r)
-            if (row0 + r < m && col0 + lane < n)
-                g[static_cast<int64_t>(row0 + r) * stride + col0 + lane] =
-                    *reinterpret_cast<const uint16_t*>(buf + staged(r, lane >> 3) + (lane & 7) * 2);
+        for (int i = 0; i < 16; ++i) {
+            const int r = i * 2 + (lane >> 4);
+            if (row0 + r < e.m && col0 + c < e.n)
+                g[r * e.out_stride] = *reinterpret_cast<const uint16_t*>(buf + staged(r, c >> 3) + (c & 7) * 2);
+        }
     }
 }
 
@@ -209,13 +278,14 @@ __device__ __forceinline__ void tile_at(const LinearParams& p, int t, int& tm, i
     tm = b * p.band + in - tn * rows;
 }
 
-template <bool kFp8>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
-    linear_pair_kernel(const __grid_constant__ LinearParams p) {
+// kSplit: one tile per cluster of p.split pairs, each pair taking a share of k (see choose_plan).
+template <bool kFp8, bool kSplit>
+__global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __grid_constant__ LinearParams p) {
     extern __shared__ char smem_raw[];
     char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     char* staging = smem + kPairStages * kPairStageBytes;
-    char* ctl = staging + 8 * kStagingBytes;
+    char* columns = staging + kEpilogueWarps * kStagingBytes;
+    char* ctl = columns + kEpilogueWarps * kColsBytes;
     const uint32_t bars = smem_u32(ctl);
     const uint32_t full = bars, empty = bars + 8 * kPairStages, acc_full = bars + 16 * kPairStages, acc_empty = acc_full + 16;
     const uint32_t drain = acc_empty + 16;
@@ -223,7 +293,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);  // [0] raised, [1] site
     int* dead = const_cast<int*>(abort_flag) + 2;                               // this block's view of the status word
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = cluster_rank();
+    const uint32_t cta = cluster_rank(), rank = cta & 1, first = cta & ~1u;  // rank in the pair; the pair's first block
+    const uint16_t both_blocks = static_cast<uint16_t>(3u << first);
     const uint32_t limit = p.wait_limit_us;
 
     if (threadIdx.x == 0) {
@@ -233,7 +304,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(acc_full + 8 * i, 1);
-            mbar_init(acc_empty + 8 * i, 16);
+            mbar_init(acc_empty + 8 * i, 2 * kEpilogueWarps);
         }
         mbar_init(drain, 1);
         fence_mbar_init();
@@ -252,15 +323,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     // Both blocks take the same decision, from what both of them saw.
-    const bool gave_up_before = (*dead | cluster_load_i32(cluster_map(smem_u32(dead), rank ^ 1))) != 0;
+    const bool gave_up_before = (*dead | cluster_load_i32(cluster_map(smem_u32(dead), cta ^ 1))) != 0;
     const int tiles = p.tiles_m * p.tiles_n;
-    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const int share = kSplit ? static_cast<int>(cta >> 1) : 0;
+    const int pair = kSplit ? blockIdx.x / (2 * p.split) : blockIdx.x >> 1, pairs = kSplit ? tiles : gridDim.x >> 1;
+    const int ks0 = kSplit ? static_cast<int>(static_cast<int64_t>(p.k_steps) * share / p.split) : 0;
+    const int ks1 = kSplit ? static_cast<int>(static_cast<int64_t>(p.k_steps) * (share + 1) / p.split) : p.k_steps;
 
     if (warp == 0) {
         if (lane == 0 && !gave_up_before && !p.test_withhold) {
             const uint32_t ring = smem_u32(smem);
             const uint32_t w_bytes = static_cast<uint32_t>(p.tile_n / 2) * kStepBytes;
-            const uint32_t full0 = cluster_map(full, 0);  // the pair's barriers are those of its first block
+            const uint32_t full0 = cluster_map(full, first);  // the pair's barriers are those of its first block
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
@@ -269,15 +343,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 tile_at(p, t, tm, tn);
                 const int row_x = tm * 256 + static_cast<int>(rank) * 128;
                 const int row_w = tn * p.tile_n + static_cast<int>(rank) * (p.tile_n / 2);
-                for (int ks = 0; ks < p.k_steps; ++ks) {
+                for (int ks = ks0; ks < ks1; ks += kSub) {
                     if (!mbar_wait(empty + 8 * stage, phase ^ 1, abort_flag, 1, limit)) {
                         ok = false;
                         break;
                     }
-                    if (rank == 0) mbar_arrive_expect_tx(full + 8 * stage, 2 * (kRowTile + w_bytes));
-                    const uint32_t dst = ring + stage * kPairStageBytes;
-                    tma_load_4d_pair(dst, &p.tm_x, full0 + 8 * stage, ks * p.k_step_elems, row_x, 0, 0);
-                    tma_load_4d_pair(dst + kRowTile, &p.tm_w, full0 + 8 * stage, ks * p.k_step_elems, row_w, 0, 0);
+                    const int subs = min(kSub, ks1 - ks);
+                    if (rank == 0) mbar_arrive_expect_tx(full + 8 * stage, subs * 2 * (kRowTile + w_bytes));
+                    uint32_t dst = ring + stage * kPairStageBytes;
+                    for (int j = 0; j < subs; ++j, dst += kPairStepBytes) {
+                        tma_load_4d_pair(dst, &p.tm_x, full0 + 8 * stage, (ks + j) * p.k_step_elems, row_x, 0, 0);
+                        tma_load_4d_pair(dst + kRowTile, &p.tm_w, full0 + 8 * stage, (ks + j) * p.k_step_elems, row_w, 0, 0);
+                    }
                     if (++stage == kPairStages) {
                         stage = 0;
                         phase ^= 1;
@@ -312,7 +389,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 }
                 tc_fence_after();
                 const uint32_t d = tmem + acc * 256;
-                for (int ks = 0; ks < p.k_steps; ++ks) {
+                for (int ks = ks0; ks < ks1; ks += kSub) {
                     if (!mbar_wait(full + 8 * stage, phase, abort_flag, 4, limit)) {
                         ok = false;
                         break;
@@ -321,116 +398,237 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                     const uint32_t a = desc_lo(ring + stage * kPairStageBytes, 16);
                     const uint32_t b = desc_lo(ring + stage * kPairStageBytes + kRowTile, 16);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)  // 32 bytes of k per MMA
-                        umma_ss_pair<kFp8>(d, a + 2 * i, b + 2 * i, kDescHiSbo1024, p.idesc, (ks | i) != 0);
-                    umma_commit_pair(empty + 8 * stage);
+                    for (int j = 0; j < kSub; ++j) {
+                        if (ks + j >= ks1) break;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)  // 32 bytes of k per MMA
+                            umma_ss_pair<kFp8>(d, a + j * (kPairStepBytes >> 4) + 2 * i, b + j * (kPairStepBytes >> 4) + 2 * i,
+                                               kDescHiSbo1024, p.idesc, ks > ks0 || (j | i) != 0);
+                    }
+                    umma_commit_pair(empty + 8 * stage, both_blocks);
                     if (++stage == kPairStages) {
                         stage = 0;
                         phase ^= 1;
                     }
                 }
-                if (ok) umma_commit_pair(acc_full + 8 * acc);
+                if (ok) umma_commit_pair(acc_full + 8 * acc, both_blocks);
                 if ((acc ^= 1) == 0) acc_phase ^= 1;
             }
             if (!ok) {  // tensor memory and the operands stay until the MMAs that were issued are over
-                umma_commit_pair(drain);
+                umma_commit_pair(drain, both_blocks);
                 mbar_wait_drain(drain, 0);
             }
         }
     } else if (warp >= 4) {
         const Epilogue& e = p.e;
-        const int quarter = warp & 3, half = (warp - 4) >> 2;
+        const int quarter = warp & 3, turn = (warp - 4) >> 2;  // rows of the tile, first unit of this warp
         char* buf = staging + (warp - 4) * kStagingBytes;
-        const uint32_t acc_empty0 = cluster_map(acc_empty, 0);
+        constexpr int kCols = kMaxUnits * kUnit;
+        float* cols = reinterpret_cast<float*>(columns + (warp - 4) * kColsBytes);  // [bias | weight scale | gate][kCols]
+        const uint32_t acc_empty0 = cluster_map(acc_empty, first);
+        const uint16_t* residual = static_cast<const uint16_t*>(e.residual);
+        uint4 ahead[2];  // the residual of the next unit
         int acc = 0;
         uint32_t acc_phase = 0;
         bool ok = !gave_up_before;
-        const int chunks = p.tile_n / 32;
+        const int units = p.tile_n / kUnit;
         for (int t = pair; t < tiles; t += pairs) {
             int tm, tn;
             tile_at(p, t, tm, tn);
             const int row0 = tm * 256 + static_cast<int>(rank) * 128 + quarter * 32;
             const int row = row0 + lane;
             const bool live = row < e.m;
+            const UnitAt out_at(e.out, e.out_stride, row0, e.m, lane), residual_at(e.residual, e.residual_stride, row0, e.m, lane);
             float xs = 1.0f;
             if (kFp8 && live) xs = __ldg(e.x_scale + static_cast<int64_t>(row) * e.x_scale_step);
+            // What the columns of this warp need is fetched while the MMAs of the tile still run.  The gate's row is
+            // taken along where all rows of the warp share it (a sample's boundary can fall between them).
             const int64_t gate_at = e.gate && live ? static_cast<int64_t>(static_cast<uint32_t>(row) / e.rows_per_gate) * e.gate_stride : 0;
-            if (ok) ok = mbar_wait(acc_full + 8 * acc, acc_phase, abort_flag, 5, limit);
-            ok = __all_sync(0xffffffffu, ok);
-            tc_fence_after();
-            for (int c = half; c < chunks; c += 2) {
-                const int col0 = tn * p.tile_n + c * 32;
-                uint32_t acc_bits[32];
-                if (ok) {
-                    tmem_ld32(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + acc * 256 + c * 32, acc_bits);
-                    if (e.residual && col0 < e.n)
-                        stage_in(buf, static_cast<const uint16_t*>(e.residual), e.residual_stride, row0, col0, e.m, e.n,
-                                 e.wide_residual, lane);
-                    tmem_wait_ld();
-                } else {
+            const int64_t gate_first = __shfl_sync(0xffffffffu, gate_at, 0);
+            const bool shared_gate = e.gate && __all_sync(0xffffffffu, !live || gate_at == gate_first);
+            __syncwarp();
+            float b2[kCols / 32] = {}, s2[kCols / 32] = {}, g2[kCols / 32] = {};  // all loads first: one trip to L2, not one for each
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) acc_bits[i] = 0x7fc00000u;  // NaN: never plausible numbers
+            for (int i = 0; i < kCols / 32; ++i) {
+                const int u = turn + kUnitWarps * (2 * i + (lane >> 4)), col = tn * p.tile_n + u * kUnit + (lane & 15);
+                if (u >= units || col >= e.n) continue;
+                if (e.bias) b2[i] = load_any(e.bias, e.bias_type, col);
+                if (kFp8) s2[i] = __ldg(e.w_scale + static_cast<int64_t>(col) * e.w_scale_step);
+                if (shared_gate) g2[i] = load_any(e.gate, e.gate_type, gate_first + col);
+            }
+#pragma unroll
+            for (int i = 0; i < kCols / 32; ++i) {
+                cols[i * 32 + lane] = b2[i];
+                if (kFp8) cols[kCols + i * 32 + lane] = s2[i];
+                cols[2 * kCols + i * 32 + lane] = g2[i];
+            }
+            if (e.residual && live)  // its way from memory to L2 also runs under the MMAs
+                for (int u = turn; u < units; u += kUnitWarps)
+                    prefetch_l2(residual + static_cast<int64_t>(row) * e.residual_stride + min(tn * p.tile_n + u * kUnit, e.n - 1));
+            __syncwarp();
+            // Values of a unit's columns in this lane's row (the j-th unit of the warp), from accumulator to output.
+            auto finish = [&](uint64_t (&v)[kUnit / 2], int j, int col0) {
+                const ulonglong2* at = reinterpret_cast<const ulonglong2*>(cols + j * kUnit);  // two pairs of columns per load
+                if constexpr (kFp8) {
+#pragma unroll
+                    for (int i = 0; i < kUnit / 4; ++i) {
+                        const ulonglong2 f = at[kCols / 4 + i];
+                        v[2 * i] = mul2(v[2 * i], mul2(f.x, both(xs)));
+                        v[2 * i + 1] = mul2(v[2 * i + 1], mul2(f.y, both(xs)));
+                    }
                 }
-                if (col0 >= e.n) continue;
-                __syncwarp();
-                uint4 old[4];
+                if (e.bias) {
+#pragma unroll
+                    for (int i = 0; i < kUnit / 4; ++i) {
+                        const ulonglong2 f = at[i];
+                        v[2 * i] = add2(v[2 * i], f.x);
+                        v[2 * i + 1] = add2(v[2 * i + 1], f.y);
+                    }
+                }
+                activate(v, e.act);
+                if (shared_gate) {
+#pragma unroll
+                    for (int i = 0; i < kUnit / 4; ++i) {
+                        const ulonglong2 f = at[kCols / 2 + i];
+                        v[2 * i] = mul2(v[2 * i], f.x);
+                        v[2 * i + 1] = mul2(v[2 * i + 1], f.y);
+                    }
+                } else if (e.gate) {
+#pragma unroll
+                    for (int q = 0; q < kUnit / 8; ++q) {
+                        float f[8];
+                        load_cols8(e.gate, e.gate_type, gate_at, col0 + q * 8, e.n, e.wide_gate, f);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v[q * 4 + i] = mul2(v[q * 4 + i], pack2(f[2 * i], f[2 * i + 1]));
+                    }
+                }
                 if (e.residual) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) old[q] = *reinterpret_cast<const uint4*>(buf + staged(lane, q));
-                    __syncwarp();
-                }
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int col = col0 + q * 8;
-                    float v[8], f[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(acc_bits[q * 8 + i]);
-                    if constexpr (kFp8) {
-                        if (e.w_scale_step) {
-                            load_cols8(e.w_scale, MINDIESD_FP32, 0, col, e.n, e.wide_cols, f);
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) v[i] *= xs * f[i];
-                        } else {
-                            const float s = xs * __ldg(e.w_scale);
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) v[i] *= s;
-                        }
-                    }
-                    if (e.bias) {
-                        load_cols8(e.bias, e.bias_type, 0, col, e.n, e.wide_cols, f);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] += f[i];
-                    }
-                    activate(v, e.act);
-                    if (e.gate) {
-                        load_cols8(e.gate, e.gate_type, gate_at, col, e.n, e.wide_cols, f);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] *= f[i];
-                    }
-                    if (e.residual) {
-                        const uint32_t w[4] = {old[q].x, old[q].y, old[q].z, old[q].w};
+                    for (int q = 0; q < kUnit / 8; ++q) {
+                        const uint4 old = *reinterpret_cast<const uint4*>(buf + staged(lane, q));
+                        const uint32_t w[4] = {old.x, old.y, old.z, old.w};
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             float lo, hi;
                             unpack_pair(w[i], e.out_fp16, lo, hi);
-                            v[2 * i] += lo;
-                            v[2 * i + 1] += hi;
+                            v[q * 4 + i] = add2(v[q * 4 + i], pack2(lo, hi));
                         }
                     }
-                    *reinterpret_cast<uint4*>(buf + staged(lane, q)) =
-                        make_uint4(pack_pair(v[0], v[1], e.out_fp16), pack_pair(v[2], v[3], e.out_fp16),
-                                   pack_pair(v[4], v[5], e.out_fp16), pack_pair(v[6], v[7], e.out_fp16));
+                    __syncwarp();
                 }
+                uint32_t w[kUnit / 2];
+                if (e.out_fp16) pack_values<true>(v, w);
+                else pack_values<false>(v, w);
+#pragma unroll
+                for (int q = 0; q < kUnit / 8; ++q)
+                    *reinterpret_cast<uint4*>(buf + staged(lane, q)) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
                 __syncwarp();
-                stage_out(buf, static_cast<uint16_t*>(e.out), e.out_stride, row0, col0, e.m, e.n, e.wide_out, lane);
+                stage_out(buf, out_at, e, row0, col0, lane);
                 __syncwarp();
+            };
+            const uint32_t tmem_rows = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+            const float nan = __uint_as_float(0x7fc00000u);  // what a wait that gave up leaves: never plausible numbers
+            if constexpr (!kSplit) {
+                if (e.residual) fetch_unit(ahead, residual_at, tn * p.tile_n + turn * kUnit, e.n, e.wide_residual, lane);
+                // The first tile starts with a pass beyond the last column, which loads and stores nothing: it brings
+                // the code below into the instruction cache while the first MMAs run.
+#pragma unroll 1
+                for (int j = t == pair ? -1 : 0, u = turn + kUnitWarps * j; u < units; ++j, u += kUnitWarps) {
+                    const int col0 = j < 0 ? e.n : tn * p.tile_n + u * kUnit;
+                    if (j == 0) {
+                        if (ok) ok = mbar_wait(acc_full + 8 * acc, acc_phase, abort_flag, 5, limit);
+                        ok = __all_sync(0xffffffffu, ok);
+                        tc_fence_after();
+                    }
+                    uint64_t v[kUnit / 2];
+                    {
+                        uint32_t bits[16];
+                        if (ok && j >= 0) {
+                            tmem_ld16(tmem_rows + acc * 256 + u * kUnit, bits);
+                            tmem_wait_ld();
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < kUnit; ++i) bits[i] = __float_as_uint(nan);
+                        }
+#pragma unroll
+                        for (int i = 0; i < kUnit / 2; ++i) v[i] = pack2(__uint_as_float(bits[2 * i]), __uint_as_float(bits[2 * i + 1]));
+                    }
+                    if (col0 >= e.n && j >= 0) continue;
+                    if (e.residual && j >= 0) {
+                        put_unit(buf, ahead, lane);
+                        __syncwarp();
+                        if (u + kUnitWarps < units)
+                            fetch_unit(ahead, residual_at, col0 + kUnitWarps * kUnit, e.n, e.wide_residual, lane);
+                    }
+                    finish(v, j < 0 ? 0 : j, col0);
+                }
+                if (units <= turn) {  // a tile with fewer units than warps: this one only hands the accumulator back
+                    if (ok) ok = mbar_wait(acc_full + 8 * acc, acc_phase, abort_flag, 5, limit);
+                    ok = __all_sync(0xffffffffu, ok);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0 && ok) mbar_arrive_cluster(acc_empty0 + 8 * acc);
+                if ((acc ^= 1) == 0) acc_phase ^= 1;
+            } else {
+                // The ring is free once the accumulator is complete: it takes this pair's partial sums, in units of
+                // 128 rows x 64 bytes whose 16-byte pieces are permuted within a row against bank conflicts.  After
+                // a wait that gave up copies may still land there, so nothing is written; the flag speaks for it.
+                const int at = quarter * 32 + lane;
+                auto piece = [&](int u, int q) { return u * 8192 + at * 64 + ((q ^ ((at >> 1) & 3)) << 4); };
+                int failed = 0;
+                // Unit j of every warp is finished by pair j mod split, which adds the pairs' sums in their order.
+                // (j = -1: the pass that brings the code into the instruction cache.)
+#pragma unroll 1
+                for (int j = -1; j <= 0 || turn + kUnitWarps * j < units; ++j) {
+                    const int u = turn + kUnitWarps * j, col0 = j < 0 ? e.n : tn * p.tile_n + u * kUnit;
+                    if (j == 0) {
+                        if (ok) ok = mbar_wait(acc_full, 0, abort_flag, 5, limit);
+                        ok = __all_sync(0xffffffffu, ok);
+                        tc_fence_after();
+                        for (int w = turn; w < units && ok; w += kUnitWarps) {
+                            uint32_t bits[16];
+                            tmem_ld16(tmem_rows + w * kUnit, bits);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int q = 0; q < 4; ++q)
+                                *reinterpret_cast<uint4*>(smem + piece(w, q)) =
+                                    make_uint4(bits[4 * q], bits[4 * q + 1], bits[4 * q + 2], bits[4 * q + 3]);
+                        }
+                        tc_fence_before();
+                        __syncwarp();
+                        cluster_sync_all();
+                        for (int i = 0; i < p.split; ++i) {
+                            failed |= cluster_load_i32(cluster_map(smem_u32(const_cast<int*>(abort_flag)), 2 * i + rank));
+                            failed |= cluster_load_i32(cluster_map(smem_u32(dead), 2 * i + rank));
+                        }
+                    }
+                    if (j >= 0 && (u >= units || j % p.split != share || col0 >= e.n)) continue;
+                    if (e.residual) fetch_unit(ahead, residual_at, col0, e.n, e.wide_residual, lane);
+                    uint64_t v[kUnit / 2];
+#pragma unroll
+                    for (int i = 0; i < kUnit / 2; ++i) v[i] = both(failed ? nan : 0.0f);
+                    for (int i = 0; i < p.split && j >= 0; ++i) {
+                        float4 part[4];
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) part[q] = cluster_load_f32x4(cluster_map(smem_u32(smem) + piece(u, q), 2 * i + rank));
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            v[2 * q] = add2(v[2 * q], pack2(part[q].x, part[q].y));
+                            v[2 * q + 1] = add2(v[2 * q + 1], pack2(part[q].z, part[q].w));
+                        }
+                    }
+                    if (e.residual) {
+                        put_unit(buf, ahead, lane);
+                        __syncwarp();
+                    }
+                    finish(v, j < 0 ? 0 : j, col0);
+                }
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0 && ok) mbar_arrive_cluster(acc_empty0 + 8 * acc);
-            if ((acc ^= 1) == 0) acc_phase ^= 1;
         }
     }
+    __syncwarp();
+    if (kSplit && warp < 4) cluster_sync_all();  // the one between the partial sums and their addition
     __syncwarp();
     tc_fence_before();
     __syncthreads();
@@ -483,6 +681,52 @@ __global__ void __launch_bounds__(kSwapThreads) linear_swap_kernel(const __grid_
     const uint32_t tmem = *tmem_slot;
     bool ok = !dead;
 
+    const Epilogue& e = p.e;
+    const int quarter = warp & 3;  // warps 2..5 cover the four quarters of the 128 lanes
+    const int channel = row_w + lane * 4;
+    float b[4] = {}, scale[4] = {};
+    // The finished values of four consecutive channels of one token.
+    auto finish = [&](float (&v)[4], int token, int first) {
+        const int64_t row = row_x + token;
+        if (kFp8) {
+            const float xs = __ldg(e.x_scale + row * e.x_scale_step);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] *= xs * scale[i];
+        }
+        uint64_t pairs[2] = {pack2(v[0] + b[0], v[1] + b[1]), pack2(v[2] + b[2], v[3] + b[3])};
+        activate(pairs, e.act);
+        unpack2(pairs[0], v[0], v[1]);
+        unpack2(pairs[1], v[2], v[3]);
+        if (e.gate) {
+            const int64_t at = static_cast<int64_t>(static_cast<uint32_t>(row) / e.rows_per_gate) * e.gate_stride + first;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (first + i < e.n) v[i] *= load_any(e.gate, e.gate_type, at + i);
+        }
+        if (e.residual) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (first + i < e.n)
+                    v[i] += load_any(e.residual, e.out_fp16 ? MINDIESD_FP16 : MINDIESD_BF16, row * e.residual_stride + first + i);
+        }
+        const uint32_t lo = pack_pair(v[0], v[1], e.out_fp16), hi = pack_pair(v[2], v[3], e.out_fp16);
+        uint16_t* o = static_cast<uint16_t*>(e.out) + row * e.out_stride + first;
+        if (e.wide_out) {  // n is a multiple of 8 then
+            if (first < e.n) *reinterpret_cast<uint2*>(o) = make_uint2(lo, hi);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (first + i < e.n) o[i] = static_cast<uint16_t>((i < 2 ? lo : hi) >> ((i & 1) * 16));
+        }
+    };
+    if (warp >= 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            b[i] = e.bias && channel + i < e.n ? load_any(e.bias, e.bias_type, channel + i) : 0.0f;
+            scale[i] = kFp8 && channel + i < e.n ? __ldg(e.w_scale + static_cast<int64_t>(channel + i) * e.w_scale_step) : 0.0f;
+        }
+    }
+
     if (warp == 0) {
         if (lane == 0 && ok && !p.test_withhold) {
             const uint32_t ring = smem_u32(smem);
@@ -533,70 +777,68 @@ __global__ void __launch_bounds__(kSwapThreads) linear_swap_kernel(const __grid_
             umma_commit(done);  // also after a wait that gave up: the MMAs that were issued must be over
             mbar_wait_drain(done, 0);
         }
-    } else if (ok) {
-        ok = mbar_wait(done, 0, abort_flag, 8, limit);
     }
-    __syncwarp();
-    // The loader's drain, the MMA thread's wait and the epilogue's wait are all over: the ring is free.
-    ok = __syncthreads_and(ok && abort_flag[0] == 0);
-    tc_fence_after();
 
-    const Epilogue& e = p.e;
-    const int quarter = warp & 3;
-    const int channel = row_w + quarter * 32 + lane;  // warps 2..5 cover the four quarters of the 128 lanes
-    const bool live = channel < e.n;
-    const bool worker = warp >= 2;
-    float bias = 0.0f, ws = 1.0f;
-    if (worker && live) {
-        if (e.bias) bias = load_any(e.bias, e.bias_type, channel);
-        if (kFp8) ws = __ldg(e.w_scale + static_cast<int64_t>(channel) * e.w_scale_step);
-    }
-    auto finish = [&](float acc, int token) {
-        const int64_t row = row_x + token;
-        float v[1] = {acc};
-        if (kFp8) v[0] *= __ldg(e.x_scale + row * e.x_scale_step) * ws;
-        if (e.bias) v[0] += bias;
-        activate(v, e.act);
-        if (e.gate)
-            v[0] *= load_any(e.gate, e.gate_type, static_cast<int64_t>(static_cast<uint32_t>(row) / e.rows_per_gate) * e.gate_stride + channel);
-        if (e.residual) v[0] += load_any(e.residual, e.out_fp16 ? MINDIESD_FP16 : MINDIESD_BF16, row * e.residual_stride + channel);
-        if (e.out_fp16) static_cast<__half*>(e.out)[row * e.out_stride + channel] = __float2half_rn(v[0]);
-        else static_cast<__nv_bfloat16*>(e.out)[row * e.out_stride + channel] = __float2bfloat16_rn(v[0]);
-    };
     const int tokens = min(p.tile_n, e.m - row_x);
-    const float bad = __uint_as_float(0x7fc00000u);
     float* partial = reinterpret_cast<float*>(smem);  // [token][128]
-    if (worker) {
-        const int lane_at = quarter * 32 + lane;
-        for (int c = 0; c < tokens; c += 8) {
-            uint32_t r[8];
-            if (ok) {
-                tmem_ld8(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + c, r);
-                tmem_wait_ld();
-            }
+    auto meet = [&] {
+        if (p.split > 1) cluster_sync_all();
+        else __syncthreads();
+    };
+    if (warp >= 2) {  // a lane takes four channels of one token
+        const uint32_t mine = smem_u32(partial) + lane * 16;
+        // The loop starts with a pass beyond the last channel, which loads and stores nothing: it brings the code
+        // below into the instruction cache while the weights are on their way.
+        int t = -1;
+#pragma unroll 1
+        do {
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (t >= 0) {  // every partial sum is on its way at once, and added in the order of the ranks
+                float4 part[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float v = ok ? __uint_as_float(r[i]) : bad;
-                if (p.split > 1) partial[(c + i) * 128 + lane_at] = v;
-                else if (live && c + i < tokens) finish(v, c + i);
+                for (int r = 0; r < 8; ++r)
+                    if (r < p.split) part[r] = cluster_load_f32x4(cluster_map(mine + t * 512, r));
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (r < p.split) {
+                        v[0] += part[r].x;
+                        v[1] += part[r].y;
+                        v[2] += part[r].z;
+                        v[3] += part[r].w;
+                    }
             }
-        }
-        tc_fence_before();
+            finish(v, t < 0 ? 0 : t, t < 0 ? e.n : channel);
+            if (t >= 0) {
+                t += p.split * 4;
+                continue;
+            }
+            if (ok) ok = mbar_wait(done, 0, abort_flag, 8, limit);
+            __syncwarp();
+            ok = __syncthreads_and(ok && abort_flag[0] == 0);  // with warps 0 and 1: the ring is free
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < tokens; c += 16) {
+                uint32_t r[16];
+                if (ok) {
+                    tmem_ld16(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + c, r);
+                    tmem_wait_ld();
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    partial[(c + i) * 128 + quarter * 32 + lane] = ok ? __uint_as_float(r[i]) : __uint_as_float(0x7fc00000u);  // NaN
+            }
+            tc_fence_before();
+            __syncwarp();
+            meet();
+            t = rank * 4 + quarter;
+        } while (t < tokens);
+    } else {
+        __syncwarp();
+        __syncthreads_and(ok && abort_flag[0] == 0);
+        meet();
     }
     __syncwarp();
-    if (p.split > 1) {
-        cluster_sync_all();
-        if (worker) {
-            const uint32_t mine = smem_u32(partial) + (quarter * 32 + lane) * 4;
-            for (int t = rank; t < tokens; t += p.split) {
-                float sum = 0.0f;
-                for (int r = 0; r < p.split; ++r) sum += cluster_load_f32(cluster_map(mine + t * 512, r));
-                if (live) finish(sum, t);
-            }
-        }
-        __syncwarp();
-        cluster_sync_all();  // the partials are read by the other blocks until here
-    }
+    if (p.split > 1) cluster_sync_all();  // the partials are read by the other blocks until here
     __syncthreads();
     if (warp == 1) tmem_dealloc(tmem, p.tmem_cols);
     if (threadIdx.x == 0) report(p, abort_flag);
@@ -607,33 +849,70 @@ __global__ void __launch_bounds__(kSwapThreads) linear_swap_kernel(const __grid_
 constexpr int kSms = 148;
 constexpr int kMaxSmem = 227 * 1024;
 
-template <bool kFp8>
-cudaError_t launch_pair(LinearParams& p, cudaStream_t stream) {
-    cudaError_t err = cudaFuncSetAttribute(linear_pair_kernel<kFp8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem);
-    if (err != cudaSuccess) return err;
-    const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
-    const int pairs = static_cast<int>(tiles < kSms / 2 ? tiles : kSms / 2);
-    linear_pair_kernel<kFp8><<<2 * pairs, kPairThreads, kPairSmem, stream>>>(p);
-    return cudaGetLastError();
-}
-
-template <bool kFp8>
-cudaError_t launch_swap(LinearParams& p, int smem, cudaStream_t stream) {
-    cudaError_t err = cudaFuncSetAttribute(linear_swap_kernel<kFp8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+template <typename Kernel>
+cudaError_t launch_clusters(Kernel kernel, const LinearParams& p, dim3 grid, int cluster, int threads, int smem, cudaStream_t stream) {
+    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (err != cudaSuccess) return err;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.split, (p.e.n + 127) / 128, (p.e.m + p.tile_n - 1) / p.tile_n);
-    cfg.blockDim = dim3(kSwapThreads, 1, 1);
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads, 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = p.split;
+    attr[0].val.clusterDim.x = cluster;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, linear_swap_kernel<kFp8>, p);
+    return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <bool kFp8>
+cudaError_t launch_pair(const LinearParams& p, cudaStream_t stream) {
+    const int tiles = p.tiles_m * p.tiles_n;
+    if (p.split > 1)
+        return launch_clusters(linear_pair_kernel<kFp8, true>, p, dim3(2 * p.split * tiles), 2 * p.split, kPairThreads, kPairSmem, stream);
+    return launch_clusters(linear_pair_kernel<kFp8, false>, p, dim3(2 * (tiles < kSms / 2 ? tiles : kSms / 2)), 2, kPairThreads,
+                           kPairSmem, stream);
+}
+
+// How a product is cut up.
+struct Plan {
+    bool swap;
+    int tile_n;         // pair: columns, swap: tokens
+    int stages;         // swap
+    int split;          // blocks (swap) or pairs (pair) that share the k of a tile
+    int band;           // pair
+};
+
+constexpr int swap_columns(int tile_n) { return tile_n <= 32 ? 32 : tile_n <= 64 ? 64 : tile_n <= 128 ? 128 : 256; }
+constexpr int swap_smem(int tile_n, int stages) { return stages * (kRowTile + tile_n * kStepBytes) + kSwapCtlBytes + 1024; }
+
+Plan choose_plan(int m, int n, int k_steps) {
+    Plan plan = {};
+    if (m <= 128) {
+        plan.swap = true;
+        plan.tile_n = (m + 15) / 16 * 16;
+        const int stage_bytes = kRowTile + plan.tile_n * kStepBytes;
+        plan.stages = (74 * 1024 - swap_smem(0, 0)) / stage_bytes;
+        if (plan.stages < 4) plan.stages = 4;
+        const int blocks = (n + 127) / 128;
+        const int slots = kSms * (kMaxSmem / (swap_smem(plan.tile_n, plan.stages) + 1024));
+        plan.split = 1;
+        while (plan.split < 8 && (plan.split + 1) * blocks <= slots && k_steps >= 2 * (plan.split + 1)) ++plan.split;
+    } else {
+        plan.tile_n = 256;
+        plan.band = 8;
+        plan.split = 1;
+    }
+    return plan;
+}
+
+template <bool kFp8>
+cudaError_t launch_swap(const LinearParams& p, cudaStream_t stream) {
+    const dim3 grid(p.split, (p.e.n + 127) / 128, (p.e.m + p.tile_n - 1) / p.tile_n);
+    return launch_clusters(linear_swap_kernel<kFp8>, p, grid, p.split, kSwapThreads, swap_smem(p.tile_n, p.stages), stream);
 }
 
 }  // namespace
@@ -691,8 +970,7 @@ extern "C" int mindiesd_linear_fwd(const mindiesd_linear_args* a, void* stream_)
     // 16-byte access: rows start on a 16-byte boundary and hold whole vectors.
     e.wide_out = aligned(a->out, 16) && e.out_stride % 8 == 0 && a->n % 8 == 0;
     e.wide_residual = a->residual && aligned(a->residual, 16) && a->residual_stride % 8 == 0 && a->n % 8 == 0;
-    e.wide_cols = aligned(a->bias, 16) && aligned(a->gate, 16) && aligned(a->weight_scale, 16) &&
-                  (!a->gate || (a->gate_stride * dtype_bytes(a->gate_dtype)) % 16 == 0);
+    e.wide_gate = a->gate && aligned(a->gate, 16) && (a->gate_stride * dtype_bytes(a->gate_dtype)) % 16 == 0;
     p.wait_limit_us = a->wait_limit_us ? a->wait_limit_us : kWaitLimitUs;
     p.test_withhold = a->test_withhold;
     p.status = device_status_word();
@@ -703,30 +981,22 @@ extern "C" int mindiesd_linear_fwd(const mindiesd_linear_args* a, void* stream_)
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     int rc;
     cudaError_t err;
-    if (a->m <= 128) {
-        p.tile_n = (a->m + 15) / 16 * 16;
-        p.tmem_cols = p.tile_n <= 32 ? 32 : p.tile_n <= 64 ? 64 : 128;
+    const Plan plan = choose_plan(a->m, a->n, p.k_steps);
+    p.tile_n = plan.tile_n;
+    p.split = plan.split;
+    if (plan.swap) {
+        p.tmem_cols = swap_columns(p.tile_n);
         p.idesc = umma_idesc(fmt, 128, p.tile_n, false, false);
-        const int stage_bytes = kRowTile + p.tile_n * kStepBytes;
-        const int budget = 74 * 1024 - 1024 - kSwapCtlBytes;
-        p.stages = budget / stage_bytes;
-        if (p.stages > kSwapMaxStages) p.stages = kSwapMaxStages;
-        if (p.stages < 4) p.stages = 4;
-        const int smem = p.stages * stage_bytes + kSwapCtlBytes + 1024;
-        const int blocks = (a->n + 127) / 128;
-        const int slots = kSms * (kMaxSmem / (smem + 1024));
-        p.split = 1;
-        while (p.split < 8 && (p.split + 1) * blocks <= slots && p.k_steps >= 2 * (p.split + 1)) ++p.split;
+        p.stages = plan.stages;
+        if ((a->n + 127) / 128 > 65535 || (a->m + p.tile_n - 1) / p.tile_n > 65535) return MINDIESD_E_CAPACITY;
         if ((rc = encode_tile_map(&p.tm_w, a->weight, a->in_dtype, a->k, a->n, 1, 1, w_strides, 128))) return rc;
         if ((rc = encode_tile_map(&p.tm_x, a->x, a->in_dtype, a->k, a->m, 1, 1, x_strides, p.tile_n))) return rc;
-        if (blocks > 65535) return MINDIESD_E_CAPACITY;
-        err = fp8 ? launch_swap<true>(p, smem, stream) : launch_swap<false>(p, smem, stream);
+        err = fp8 ? launch_swap<true>(p, stream) : launch_swap<false>(p, stream);
     } else {
-        p.tile_n = 256;
         p.tiles_m = (a->m + 255) / 256;
         p.tiles_n = (a->n + p.tile_n - 1) / p.tile_n;
         if (static_cast<int64_t>(p.tiles_m) * p.tiles_n > 0x3fffffff) return MINDIESD_E_CAPACITY;
-        p.band = 8;
+        p.band = plan.band;
         p.idesc = umma_idesc(fmt, 256, p.tile_n, false, false);
         if ((rc = encode_tile_map(&p.tm_x, a->x, a->in_dtype, a->k, a->m, 1, 1, x_strides, 128))) return rc;
         if ((rc = encode_tile_map(&p.tm_w, a->weight, a->in_dtype, a->k, a->n, 1, 1, w_strides, p.tile_n / 2))) return rc;

@@ -830,47 +830,54 @@ at::Tensor as_rows(const at::Tensor& x, int64_t* rows, int64_t* stride) {
     return x;
 }
 
-std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_cuda(const at::Tensor& x, const c10::optional<at::Tensor>& weight,
-                                                                 const c10::optional<at::Tensor>& residual, double eps,
-                                                                 bool quant, bool quant_only) {
-    TORCH_CHECK(x.is_cuda() && x.dim() >= 1 && x.size(-1) > 0, "add_rms_norm: x must be a CUDA tensor [..., D]");
+bool records_gradients(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+
+using MaybeTensor = c10::optional<at::Tensor>;
+
+std::tuple<at::Tensor, MaybeTensor, MaybeTensor> add_rms_norm_cuda(const at::Tensor& x, const MaybeTensor& weight,
+                                                                   const MaybeTensor& residual, double eps, bool quant,
+                                                                   bool quant_only) {
+    const at::ScalarType type = x.scalar_type();
+    TORCH_CHECK(x.is_cuda() && x.dim() >= 1 && x.size(-1) > 0 && !records_gradients(x), "add_rms_norm: x must be a CUDA tensor [..., D]");
+    TORCH_CHECK(type == at::kBFloat16 || type == at::kHalf || type == at::kFloat, "add_rms_norm: x must be bf16, fp16 or fp32");
+    TORCH_CHECK(eps > 0 && eps < 1e30, "add_rms_norm: eps must be positive");
     const int64_t d = x.size(-1);
     TORCH_CHECK(d <= std::numeric_limits<int32_t>::max(), "add_rms_norm: D is too large");
     mindiesd_norm_args a = {};
     at::Tensor xr = as_rows(x, &a.rows, &a.x_stride);
     at::Tensor rr, wr, residual_out, scales;
-    at::Tensor out = at::empty(x.sizes(), x.options().dtype(quant ? at::kFloat8_e4m3fn : x.scalar_type()));
-    a.dtype = a.residual_dtype = a.weight_dtype = dtype_code(x.scalar_type());
+    at::Tensor out = at::empty(x.sizes(), x.options().dtype(quant ? at::kFloat8_e4m3fn : type));
+    a.dtype = a.residual_dtype = a.weight_dtype = dtype_code(type);
     a.dim = static_cast<int32_t>(d);
     if (weight.has_value()) {
-        wr = weight.value().contiguous();
-        TORCH_CHECK(wr.is_cuda() && wr.device() == x.device() && wr.dim() == 1 && wr.size(0) == d,
-                    "add_rms_norm: weight must be a tensor [D] on the device of x");
+        const at::Tensor& w = weight.value();
+        TORCH_CHECK(w.is_cuda() && w.device() == x.device() && w.dim() == 1 && w.size(0) == d &&
+                        (w.scalar_type() == type || w.scalar_type() == at::kFloat) && !records_gradients(w),
+                    "add_rms_norm: weight must be [D] on the device of x, in its type or fp32");
+        wr = w.contiguous();
         a.weight = wr.data_ptr();
         a.weight_dtype = dtype_code(wr.scalar_type());
     }
     if (residual.has_value()) {
         const at::Tensor& r = residual.value();
-        TORCH_CHECK(r.is_cuda() && r.device() == x.device() && r.sizes() == x.sizes(),
-                    "add_rms_norm: residual must have the shape and the device of x");
+        TORCH_CHECK(r.is_cuda() && r.device() == x.device() && r.sizes() == x.sizes() &&
+                        (r.scalar_type() == type || r.scalar_type() == at::kFloat) && !records_gradients(r),
+                    "add_rms_norm: residual must have the shape and the device of x, in its type or fp32");
         int64_t rows = 0;
         rr = as_rows(r, &rows, &a.residual_stride);
         residual_out = at::empty(r.sizes(), r.options());
         a.residual = rr.data_ptr();
         a.residual_out = residual_out.data_ptr();
         a.residual_dtype = dtype_code(r.scalar_type());
-    } else {
-        residual_out = at::empty({0}, x.options());
     }
     if (quant) {
         std::vector<int64_t> shape = x.sizes().vec();
         shape.back() = 1;
         scales = at::empty(shape, x.options().dtype(at::kFloat));
         a.scales = scales.data_ptr<float>();
-    } else {
-        scales = at::empty({0}, x.options().dtype(at::kFloat));
     }
-    if (a.rows == 0) return std::make_tuple(out, scales, residual_out);
+    auto made = [](const at::Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); };
+    if (a.rows == 0) return {out, made(scales), made(residual_out)};
     a.x = xr.data_ptr();
     a.out = out.data_ptr();
     a.out_dtype = quant ? MINDIESD_E4M3 : a.dtype;
@@ -878,7 +885,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_cuda(const at::Tenso
     a.eps = static_cast<float>(eps);
     c10::cuda::CUDAGuard guard(x.device());
     check_rc(mindiesd_add_rms_norm(&a, stream_of(x)), "mindiesd_add_rms_norm");
-    return std::make_tuple(out, scales, residual_out);
+    return {out, made(scales), made(residual_out)};
 }
 
 // ---- matrix product with bias, activation, gate and residual ------------------------------------------------
@@ -895,60 +902,86 @@ at::Tensor as_tma_rows(const at::Tensor& x, int64_t* rows, int64_t* stride) {
     return wide;
 }
 
+int activation_code(c10::string_view name) {
+    if (name == "none") return MINDIESD_ACT_NONE;
+    if (name == "relu") return MINDIESD_ACT_RELU;
+    if (name == "silu") return MINDIESD_ACT_SILU;
+    if (name == "gelu") return MINDIESD_ACT_GELU;
+    TORCH_CHECK(name == "gelu_tanh", "linear_fwd: unknown activation ", name);
+    return MINDIESD_ACT_GELU_TANH;
+}
+
 at::Tensor linear_fwd_cuda(const at::Tensor& x, const at::Tensor& weight, const c10::optional<at::Tensor>& bias,
                            const c10::optional<at::Tensor>& residual, const c10::optional<at::Tensor>& gate,
                            const c10::optional<at::Tensor>& x_scale, const c10::optional<at::Tensor>& weight_scale,
-                           int64_t activation, at::ScalarType out_dtype) {
-    TORCH_CHECK(x.is_cuda() && weight.is_cuda() && x.device() == weight.device() && x.scalar_type() == weight.scalar_type(),
-                "linear_fwd: x and weight must be CUDA tensors of one device and one dtype");
+                           c10::string_view activation, c10::optional<at::ScalarType> out_dtype_) {
+    const at::ScalarType type = x.scalar_type();
+    const bool fp8 = type == at::kFloat8_e4m3fn;
+    TORCH_CHECK(fp8 || type == at::kBFloat16 || type == at::kHalf, "linear_fwd: x must be bf16, fp16 or e4m3");
+    auto usable = [&](const at::Tensor& t) { return t.is_cuda() && t.device() == x.device() && !records_gradients(t); };
+    auto is_float = [](const at::Tensor& t) {
+        return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf || t.scalar_type() == at::kFloat;
+    };
+    TORCH_CHECK(usable(x) && usable(weight) && weight.scalar_type() == type, "linear_fwd: x and weight must be CUDA tensors of one device and one dtype");
     TORCH_CHECK(x.dim() >= 1 && weight.dim() == 2 && x.size(-1) == weight.size(1) && weight.size(0) > 0 && weight.size(1) > 0,
                 "linear_fwd: x must be [..., K] and weight [N, K]");
     const int64_t n = weight.size(0), k = weight.size(1), m = x.numel() / k;
     constexpr int64_t kMost = std::numeric_limits<int32_t>::max();
     TORCH_CHECK(m <= kMost && n <= kMost && k <= kMost, "linear_fwd: too many rows or columns");
+    const at::ScalarType out_dtype = out_dtype_.has_value()     ? out_dtype_.value()
+                                     : !fp8                     ? type
+                                     : residual.has_value()     ? residual.value().scalar_type()
+                                                                : at::kBFloat16;
+    TORCH_CHECK(out_dtype == at::kBFloat16 || out_dtype == at::kHalf, "linear_fwd: the output must be bf16 or fp16");
+    TORCH_CHECK(x_scale.has_value() == fp8 && weight_scale.has_value() == fp8, "linear_fwd: scales belong to e4m3 operands, which need both");
     std::vector<int64_t> shape = x.sizes().vec();
     shape.back() = n;
     at::Tensor out = at::empty(shape, x.options().dtype(out_dtype));
     mindiesd_linear_args a = {};
     at::Tensor br, rr, gr, xsr, wsr;
-    auto on_device = [&](const at::Tensor& t) { return t.is_cuda() && t.device() == x.device(); };
     if (bias.has_value()) {
-        br = bias.value().contiguous();
-        TORCH_CHECK(on_device(br) && br.dim() == 1 && br.size(0) == n, "linear_fwd: bias must be [N] on the device of x");
+        const at::Tensor& t = bias.value();
+        TORCH_CHECK(usable(t) && is_float(t) && t.dim() == 1 && t.size(0) == n, "linear_fwd: bias must be [N] on the device of x");
+        br = t.contiguous();
         a.bias = br.data_ptr();
         a.bias_dtype = dtype_code(br.scalar_type());
     }
     if (residual.has_value()) {
-        TORCH_CHECK(on_device(residual.value()) && residual.value().sizes() == out.sizes() && residual.value().scalar_type() == out_dtype,
+        const at::Tensor& t = residual.value();
+        TORCH_CHECK(usable(t) && t.sizes() == out.sizes() && t.scalar_type() == out_dtype,
                     "linear_fwd: residual must have the shape, the dtype and the device of the output");
         int64_t rows = 0;
-        rr = as_rows(residual.value(), &rows, &a.residual_stride);
+        rr = as_rows(t, &rows, &a.residual_stride);
         a.residual = rr.data_ptr();
     }
     if (gate.has_value()) {
-        const at::Tensor& g = gate.value();
-        TORCH_CHECK(on_device(g) && g.dim() >= 1 && g.size(-1) == n, "linear_fwd: gate must be [N] or [B, 1, N] on the device of x");
+        const at::Tensor& t = gate.value();
+        TORCH_CHECK(usable(t) && is_float(t) && t.dim() >= 1 && t.size(-1) == n &&
+                        (t.numel() == n || (t.dim() >= 2 && x.dim() >= 2 && t.size(0) == x.size(0) && t.numel() == x.size(0) * n)),
+                    "linear_fwd: gate must be [N] or [B, 1, N] on the device of x, B its first dimension");
         int64_t rows = 0;
-        gr = as_rows(g, &rows, &a.gate_stride);
-        TORCH_CHECK(rows == 1 || (x.dim() >= 2 && rows == x.size(0)), "linear_fwd: one gate row, or one per entry of x's first dimension");
+        gr = as_rows(t, &rows, &a.gate_stride);
         a.gate = gr.data_ptr();
         a.gate_dtype = dtype_code(gr.scalar_type());
         a.rows_per_gate = static_cast<int32_t>(rows > 0 && m > 0 ? m / rows : 1);
     }
-    if (x_scale.has_value()) {
-        xsr = x_scale.value().contiguous();
-        TORCH_CHECK(on_device(xsr) && xsr.scalar_type() == at::kFloat && (xsr.numel() == m || xsr.numel() == 1),
-                    "linear_fwd: x_scale must be fp32, one value per row of x or one in all");
-        a.x_scale = xsr.data_ptr<float>();
-        a.x_scale_single = xsr.numel() == 1;
+    auto scales = [&](const at::Tensor& t, at::IntArrayRef lead, at::Tensor& keep, const float** ptr, int32_t* single) {
+        bool fits = t.numel() == 1;
+        if (!fits) {  // the rows' own shape, with or without a last dimension of one
+            const int64_t dims = static_cast<int64_t>(lead.size());
+            fits = t.dim() == dims || (t.dim() == dims + 1 && t.size(-1) == 1);
+            for (int64_t i = 0; fits && i < dims; ++i) fits = t.size(i) == lead[i];
+        }
+        TORCH_CHECK(fits && usable(t) && t.scalar_type() == at::kFloat, "linear_fwd: scales must be fp32, one value per row or one in all");
+        keep = t.contiguous();
+        *ptr = keep.data_ptr<float>();
+        *single = keep.numel() == 1;
+    };
+    if (fp8) {
+        scales(x_scale.value(), x.sizes().slice(0, x.dim() - 1), xsr, &a.x_scale, &a.x_scale_single);
+        scales(weight_scale.value(), weight.sizes().slice(0, 1), wsr, &a.weight_scale, &a.weight_scale_single);
     }
-    if (weight_scale.has_value()) {
-        wsr = weight_scale.value().contiguous();
-        TORCH_CHECK(on_device(wsr) && wsr.scalar_type() == at::kFloat && (wsr.numel() == n || wsr.numel() == 1),
-                    "linear_fwd: weight_scale must be fp32, one value per row of weight or one in all");
-        a.weight_scale = wsr.data_ptr<float>();
-        a.weight_scale_single = wsr.numel() == 1;
-    }
+    const int act = activation_code(activation);
     if (m == 0) return out;
     c10::cuda::CUDAGuard guard(x.device());
     int64_t rows_x = 0, rows_w = 0;
@@ -962,7 +995,7 @@ at::Tensor linear_fwd_cuda(const at::Tensor& x, const at::Tensor& weight, const 
     a.k = static_cast<int32_t>(k);
     a.in_dtype = dtype_code(x.scalar_type());
     a.out_dtype = dtype_code(out_dtype);
-    a.activation = static_cast<int32_t>(activation);
+    a.activation = act;
     check_rc(mindiesd_linear_fwd(&a, stream_of(x)), "mindiesd_linear_fwd");
     return out;
 }
@@ -1026,10 +1059,10 @@ TORCH_LIBRARY(mindiesd, m) {
         "float scale, int k_block, int v_block, ScalarType out_dtype) -> Tensor");
     m.def(
         "add_rms_norm(Tensor x, Tensor? weight, Tensor? residual, float eps, bool quant, bool quant_only) "
-        "-> (Tensor, Tensor, Tensor)");
+        "-> (Tensor, Tensor?, Tensor?)");
     m.def(
         "linear_fwd(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, Tensor? gate, Tensor? x_scale, "
-        "Tensor? weight_scale, int activation, ScalarType out_dtype) -> Tensor");
+        "Tensor? weight_scale, str activation='none', ScalarType? out_dtype=None) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(mindiesd, CUDA, m) {

@@ -216,10 +216,13 @@ def _fp8_attention_fake(query, key, value, q_scale, k_scale, v_scale, scale, k_b
 @register_ops.register_mindie_fake_op("add_rms_norm")
 def _add_rms_norm_fake(x, weight, residual, eps, quant, quant_only):
     out = x.new_empty(x.shape, dtype=torch.float8_e4m3fn if quant else x.dtype)
-    scales = x.new_empty([*x.shape[:-1], 1] if quant else [0], dtype=torch.float32)
-    return out, scales, x.new_empty([0]) if residual is None else residual.new_empty(residual.shape)
+    scales = x.new_empty([*x.shape[:-1], 1], dtype=torch.float32) if quant else None
+    return out, scales, None if residual is None else residual.new_empty(residual.shape)
 
 
 @register_ops.register_mindie_fake_op("linear_fwd")
-def _linear_fwd_fake(x, weight, bias, residual, gate, x_scale, weight_scale, activation, out_dtype):
+def _linear_fwd_fake(x, weight, bias, residual, gate, x_scale, weight_scale, activation="none", out_dtype=None):
+    if out_dtype is None:
+        fp8 = x.dtype == torch.float8_e4m3fn
+        out_dtype = x.dtype if not fp8 else residual.dtype if residual is not None else torch.bfloat16
     return x.new_empty([*x.shape[:-1], weight.shape[0]], dtype=out_dtype)

@@ -15,6 +15,7 @@ from .._cabi import ACTIVATIONS
 from ..utils.exception import ParametersInvalid
 from ..utils.status import checked
 
+_op = torch.ops.mindiesd.linear_fwd.default
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 
 
@@ -28,19 +29,9 @@ def _check_optional(name, t, x):
     _want(t.device == x.device, f"The input {name} must be on {x.device}, but it is on {t.device}.")
 
 
-def linear_forward(x, weight, bias=None, activation="none", residual=None, gate=None, x_scale=None, weight_scale=None,
-                   out_dtype=None):
-    """out = residual + gate * act(x @ weight.T * x_scale * weight_scale + bias), accumulated and finished in fp32
-    and rounded once.
-
-    x [..., K], weight [N, K]: both bf16, both fp16 or both e4m3.  Rows whose start and stride are multiples of 16
-    bytes are read in place; others are copied first.
-    bias: [N], bf16, fp16 or fp32.  activation: "none", "relu", "silu", "gelu" (erf) or "gelu_tanh".
-    gate: [N], or [B, N] / [B, 1, .., N] with B the first dimension of x; bf16, fp16 or fp32.
-    residual: [..., N] in the output's type.
-    x_scale, weight_scale: e4m3 operands only, where both are required: fp32, one value per row ([..., 1] or [...]
-    for x, [N] or [N, 1] for weight) or one in all.
-    out_dtype: bfloat16 or float16; by default the type of x, for e4m3 operands that of the residual or bfloat16."""
+def _explain(x, weight, bias, activation, residual, gate, x_scale, weight_scale, out_dtype):
+    """Raises ParametersInvalid for arguments the operator does not take.  The operator makes the same checks on
+    the way to the kernel; this says what was wrong, and costs a valid call nothing."""
     for name, t in (("x", x), ("weight", weight)):
         _want(isinstance(t, torch.Tensor), f"The data type of input {name} must be torch.Tensor, but got {type(t)}.")
     _want(weight.dim() == 2 and x.dim() >= 1 and x.shape[-1] == weight.shape[1] and weight.shape[0] > 0 and weight.shape[1] > 0,
@@ -81,5 +72,26 @@ def linear_forward(x, weight, bias=None, activation="none", residual=None, gate=
         _want(x_scale is None and weight_scale is None, "x_scale and weight_scale belong to e4m3 operands.")
     refuse_gradients("linear_forward", x, weight, bias, residual, gate, x_scale, weight_scale)
     _want(x.is_cuda or x.is_meta, f"linear_forward runs on a CUDA device, but x is on {x.device}.")
-    return checked(torch.ops.mindiesd.linear_fwd(x, weight, bias, residual, gate, x_scale, weight_scale,
-                                                 ACTIVATIONS[activation], out_dtype), "linear_forward")
+
+
+def linear_forward(x, weight, bias=None, activation="none", residual=None, gate=None, x_scale=None, weight_scale=None,
+                   out_dtype=None):
+    """out = residual + gate * act(x @ weight.T * x_scale * weight_scale + bias), accumulated and finished in fp32
+    and rounded once.
+
+    x [..., K], weight [N, K]: both bf16, both fp16 or both e4m3.  Rows whose start and stride are multiples of 16
+    bytes are read in place; others are copied first.
+    bias: [N], bf16, fp16 or fp32.  activation: "none", "relu", "silu", "gelu" (erf) or "gelu_tanh".
+    gate: [N], or [B, N] / [B, 1, .., N] with B the first dimension of x; bf16, fp16 or fp32.
+    residual: [..., N] in the output's type.
+    x_scale, weight_scale: e4m3 operands only, where both are required: fp32, one value per row ([..., 1] or [...]
+    for x, [N] or [N, 1] for weight) or one in all.
+    out_dtype: bfloat16 or float16; by default the type of x, for e4m3 operands that of the residual or bfloat16."""
+    try:
+        if x.is_cuda:
+            return checked(_op(x, weight, bias, residual, gate, x_scale, weight_scale, activation, out_dtype), "linear_forward")
+    except (RuntimeError, TypeError, AttributeError):
+        _explain(x, weight, bias, activation, residual, gate, x_scale, weight_scale, out_dtype)
+        raise
+    _explain(x, weight, bias, activation, residual, gate, x_scale, weight_scale, out_dtype)
+    return _op(x, weight, bias, residual, gate, x_scale, weight_scale, activation, out_dtype)  # shapes only (meta tensors)

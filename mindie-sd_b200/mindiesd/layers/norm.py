@@ -11,6 +11,7 @@ import torch
 from . import _custom_ops  # noqa: F401  (registers the fake implementations)
 from ..utils.exception import ParametersInvalid
 
+_op = torch.ops.mindiesd.add_rms_norm.default
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
@@ -22,7 +23,9 @@ def refuse_gradients(where, *tensors):
                                         "torch.inference_mode().")
 
 
-def _check(where, x, weight, residual, eps):
+def _explain(where, x, weight, residual, eps):
+    """Raises ParametersInvalid for arguments the operator does not take.  The operator makes the same checks on
+    the way to the kernel; this says what was wrong, and costs a valid call nothing."""
     if not isinstance(x, torch.Tensor):
         raise ParametersInvalid(f"The data type of input x must be torch.Tensor, but got {type(x)}.")
     if x.dim() < 1 or x.shape[-1] < 1:
@@ -52,14 +55,24 @@ def _check(where, x, weight, residual, eps):
         raise ParametersInvalid(f"{where} runs on a CUDA device, but x is on {x.device}.")
 
 
+def _run(where, x, weight, residual, eps, quant):
+    try:
+        if x.is_cuda:
+            return _op(x, weight, residual, eps, quant, False)
+    except (RuntimeError, TypeError, AttributeError):
+        _explain(where, x, weight, residual, eps)
+        raise
+    _explain(where, x, weight, residual, eps)
+    return _op(x, weight, residual, eps, quant, False)  # shapes only (meta tensors)
+
+
 def add_rms_norm(x, weight=None, residual=None, eps=1e-6):
     """y = v * weight / sqrt(mean(v^2) + eps) over the last dimension, with v = x + residual in fp32 (v = x
     without a residual) and one rounding to the type of x.  x: [..., D] bf16, fp16 or fp32; weight [D] (None:
     ones) and residual [..., D] in the type of x or fp32.  Returns y, or (y, v rounded to the residual's type)
     when a residual is given.  Leading dimensions that share one row stride (slices of a packed projection)
     are read in place."""
-    _check("add_rms_norm", x, weight, residual, eps)
-    y, _, total = torch.ops.mindiesd.add_rms_norm(x, weight, residual, eps, False, False)
+    y, _, total = _run("add_rms_norm", x, weight, residual, eps, False)
     return y if residual is None else (y, total)
 
 
@@ -67,6 +80,5 @@ def add_rms_norm_quant(x, weight=None, residual=None, eps=1e-6):
     """The same norm with its output in e4m3 and one scale per token, taken on the fp32 values: returns
     (e4m3 [..., D], fp32 scales [..., 1]), with the residual's sum as a third where one is given; real value =
     stored * scale, scale = max|y| / 448 (1 for a token of zeros, NaN for one that holds a NaN or an infinity)."""
-    _check("add_rms_norm_quant", x, weight, residual, eps)
-    q, scale, total = torch.ops.mindiesd.add_rms_norm(x, weight, residual, eps, True, False)
+    q, scale, total = _run("add_rms_norm_quant", x, weight, residual, eps, True)
     return (q, scale) if residual is None else (q, scale, total)

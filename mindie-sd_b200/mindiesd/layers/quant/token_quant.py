@@ -5,11 +5,10 @@ import torch
 from ..norm import refuse_gradients
 from ...utils.exception import ParametersInvalid
 
+_op = torch.ops.mindiesd.add_rms_norm.default
 
-def token_quant_preprocess(input_tensor):
-    """input_tensor: [..., D] bf16, fp16 or fp32.  Returns (e4m3 [..., D], fp32 scales [..., 1]); real = stored *
-    scale, scale = absmax / 448 of the token (1 for a token of zeros).  Rows of a weight matrix [N, K] quantised
-    this way have one scale per output channel."""
+
+def _explain(input_tensor):
     if not isinstance(input_tensor, torch.Tensor):
         raise ParametersInvalid(f"The data type of input_tensor must be torch.Tensor, but got {type(input_tensor)}.")
     if input_tensor.dim() < 1 or input_tensor.shape[-1] < 1:
@@ -21,5 +20,17 @@ def token_quant_preprocess(input_tensor):
     if not input_tensor.is_cuda and not input_tensor.is_meta:
         raise ParametersInvalid(f"token_quant_preprocess runs on a CUDA device, but input_tensor is on "
                                 f"{input_tensor.device}.")
-    quant, scale, _ = torch.ops.mindiesd.add_rms_norm(input_tensor, None, None, 1.0, True, True)
-    return quant, scale
+
+
+def token_quant_preprocess(input_tensor):
+    """input_tensor: [..., D] bf16, fp16 or fp32.  Returns (e4m3 [..., D], fp32 scales [..., 1]); real = stored *
+    scale, scale = absmax / 448 of the token (1 for a token of zeros).  Rows of a weight matrix [N, K] quantised
+    this way have one scale per output channel."""
+    try:
+        if input_tensor.is_cuda:
+            return _op(input_tensor, None, None, 1.0, True, True)[:2]
+    except (RuntimeError, AttributeError):
+        _explain(input_tensor)
+        raise
+    _explain(input_tensor)
+    return _op(input_tensor, None, None, 1.0, True, True)[:2]  # shapes only (meta tensors)
