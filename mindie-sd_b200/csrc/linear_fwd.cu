@@ -2,7 +2,7 @@
 //   x [m, k], w [n, k] (both k-contiguous), bf16 / fp16 / e4m3 operands, fp32 accumulation, one rounding of the result.
 //
 // Two kernels.  Both stream 128-byte wide tiles of x and w through a ring of shared-memory stages filled by a TMA
-// thread, and one thread issues tcgen05 MMAs into tensor memory.
+// warp, and one warp issues tcgen05 MMAs into tensor memory.
 //
 // `linear_pair_kernel` (many rows): persistent, two thread blocks (a cluster on neighbouring SMs) work on one
 // 256 x tile_n tile with two-SM MMAs, so each SM fetches 128 rows of x and only HALF of the tile's rows of w: 32 KB
@@ -50,7 +50,8 @@ struct LinearParams {
     int k_steps, k_step_elems;
     int tile_n;                    // pair kernel: columns of a tile; swap kernel: tokens of a tile
     int tiles_m, tiles_n, band;    // pair kernel: tiles are walked in bands of `band` row tiles
-    int stages, tmem_cols, split;  // swap kernel
+    int stages;
+    int tmem_cols, split;  // swap kernel
     uint32_t idesc;
     uint32_t wait_limit_us;
     int test_withhold;
@@ -191,9 +192,8 @@ __device__ __forceinline__ void report(const LinearParams& p, const volatile int
 constexpr int kEpilogueWarps = 16;
 constexpr int kPairThreads = 128 + 32 * kEpilogueWarps;  // warps: 0 loader, 1 MMA, 2 tensor memory, 3 idle, 4.. epilogue
 constexpr int kSub = 2;  // k steps per ring stage: one barrier round trip and one commit for eight MMAs
-constexpr int kPairStages = 6 / kSub;
-constexpr int kPairStepBytes = 2 * kRowTile;
-constexpr int kPairStageBytes = kSub * kPairStepBytes;
+constexpr int kRingBytes = 6 * 2 * kRowTile;  // pair kernel: three stages of 256-column tiles, more of narrower ones
+constexpr int kPairMaxStages = 8;
 // The epilogue works in units of 32 rows x 16 columns.  Four warps share a quarter of the tile's rows and take its
 // units in turn: with two warps of 32-column units a 256-column tile left 4 us of epilogue after its last MMA, and
 // the latency of one warp's instructions, not their number, was what it waited for.
@@ -202,7 +202,7 @@ constexpr int kUnitWarps = kEpilogueWarps / 4;
 constexpr int kMaxUnits = 256 / kUnit / kUnitWarps;  // of one warp in one tile
 constexpr int kStagingBytes = 32 * kUnit * 2;        // per warp: one unit of two-byte values
 constexpr int kColsBytes = 3 * kMaxUnits * kUnit * 4;  // per warp: bias, weight scale and gate of its columns as fp32
-constexpr int kPairSmem = kPairStages * kPairStageBytes + kEpilogueWarps * (kStagingBytes + kColsBytes) + 256 + 1024;
+constexpr int kPairSmem = kRingBytes + kEpilogueWarps * (kStagingBytes + kColsBytes) + 256 + 1024;
 static_assert(kPairSmem <= 227 * 1024, "shared memory of the pair kernel");
 
 // Offset of 16-byte piece c of row r in a warp's staging buffer; the exclusive or keeps both the row-wise writes and
@@ -278,27 +278,25 @@ __device__ __forceinline__ void tile_at(const LinearParams& p, int t, int& tm, i
     tm = b * p.band + in - tn * rows;
 }
 
-// kSplit: one tile per cluster of p.split pairs, each pair taking a share of k (see choose_plan).
-template <bool kFp8, bool kSplit>
+template <bool kFp8>
 __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __grid_constant__ LinearParams p) {
     extern __shared__ char smem_raw[];
     char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    char* staging = smem + kPairStages * kPairStageBytes;
+    char* staging = smem + kRingBytes;
     char* columns = staging + kEpilogueWarps * kStagingBytes;
     char* ctl = columns + kEpilogueWarps * kColsBytes;
     const uint32_t bars = smem_u32(ctl);
-    const uint32_t full = bars, empty = bars + 8 * kPairStages, acc_full = bars + 16 * kPairStages, acc_empty = acc_full + 16;
+    const uint32_t full = bars, empty = bars + 8 * kPairMaxStages, acc_full = bars + 16 * kPairMaxStages, acc_empty = acc_full + 16;
     const uint32_t drain = acc_empty + 16;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctl + 16 * kPairStages + 40);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctl + 16 * kPairMaxStages + 40);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);  // [0] raised, [1] site
     int* dead = const_cast<int*>(abort_flag) + 2;                               // this block's view of the status word
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t cta = cluster_rank(), rank = cta & 1, first = cta & ~1u;  // rank in the pair; the pair's first block
-    const uint16_t both_blocks = static_cast<uint16_t>(3u << first);
+    const uint32_t rank = cluster_rank();
     const uint32_t limit = p.wait_limit_us;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kPairStages; ++i) {
+        for (int i = 0; i < p.stages; ++i) {
             mbar_init(full + 8 * i, 1);
             mbar_init(empty + 8 * i, 1);
         }
@@ -323,18 +321,16 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     // Both blocks take the same decision, from what both of them saw.
-    const bool gave_up_before = (*dead | cluster_load_i32(cluster_map(smem_u32(dead), cta ^ 1))) != 0;
+    const bool gave_up_before = (*dead | cluster_load_i32(cluster_map(smem_u32(dead), rank ^ 1))) != 0;
     const int tiles = p.tiles_m * p.tiles_n;
-    const int share = kSplit ? static_cast<int>(cta >> 1) : 0;
-    const int pair = kSplit ? blockIdx.x / (2 * p.split) : blockIdx.x >> 1, pairs = kSplit ? tiles : gridDim.x >> 1;
-    const int ks0 = kSplit ? static_cast<int>(static_cast<int64_t>(p.k_steps) * share / p.split) : 0;
-    const int ks1 = kSplit ? static_cast<int>(static_cast<int64_t>(p.k_steps) * (share + 1) / p.split) : p.k_steps;
+    const uint32_t step_bytes = kRowTile + static_cast<uint32_t>(p.tile_n / 2) * kStepBytes;  // of one block
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
     if (warp == 0) {
-        if (lane == 0 && !gave_up_before && !p.test_withhold) {
+        if (!gave_up_before && !p.test_withhold) {
+            const bool one = elect_one();
             const uint32_t ring = smem_u32(smem);
-            const uint32_t w_bytes = static_cast<uint32_t>(p.tile_n / 2) * kStepBytes;
-            const uint32_t full0 = cluster_map(full, first);  // the pair's barriers are those of its first block
+            const uint32_t full0 = cluster_map(full, 0);  // the pair's barriers are those of its first block
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
@@ -343,19 +339,19 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
                 tile_at(p, t, tm, tn);
                 const int row_x = tm * 256 + static_cast<int>(rank) * 128;
                 const int row_w = tn * p.tile_n + static_cast<int>(rank) * (p.tile_n / 2);
-                for (int ks = ks0; ks < ks1; ks += kSub) {
-                    if (!mbar_wait(empty + 8 * stage, phase ^ 1, abort_flag, 1, limit)) {
-                        ok = false;
-                        break;
+                for (int ks = 0; ks < p.k_steps; ks += kSub) {
+                    ok = mbar_wait_warp(empty + 8 * stage, phase ^ 1, abort_flag, 1, limit);
+                    if (!ok) break;
+                    const int subs = min(kSub, p.k_steps - ks);
+                    if (one) {
+                        if (rank == 0) mbar_arrive_expect_tx(full + 8 * stage, subs * 2 * step_bytes);
+                        uint32_t dst = ring + stage * kSub * step_bytes;
+                        for (int j = 0; j < subs; ++j, dst += step_bytes) {
+                            tma_load_4d_pair(dst, &p.tm_x, full0 + 8 * stage, (ks + j) * p.k_step_elems, row_x, 0, 0);
+                            tma_load_4d_pair(dst + kRowTile, &p.tm_w, full0 + 8 * stage, (ks + j) * p.k_step_elems, row_w, 0, 0);
+                        }
                     }
-                    const int subs = min(kSub, ks1 - ks);
-                    if (rank == 0) mbar_arrive_expect_tx(full + 8 * stage, subs * 2 * (kRowTile + w_bytes));
-                    uint32_t dst = ring + stage * kPairStageBytes;
-                    for (int j = 0; j < subs; ++j, dst += kPairStepBytes) {
-                        tma_load_4d_pair(dst, &p.tm_x, full0 + 8 * stage, (ks + j) * p.k_step_elems, row_x, 0, 0);
-                        tma_load_4d_pair(dst + kRowTile, &p.tm_w, full0 + 8 * stage, (ks + j) * p.k_step_elems, row_w, 0, 0);
-                    }
-                    if (++stage == kPairStages) {
+                    if (++stage == p.stages) {
                         stage = 0;
                         phase ^= 1;
                     }
@@ -364,58 +360,58 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
             // Nothing of this block's may be in flight when it exits: every stage that was filled has been
             // consumed (the release also tells that the loads landed), or, after a wait gave up, has landed.
             // (The barriers of a stage that was never filled let both waits pass.)
-            for (int i = 0; i < kPairStages; ++i) {
+            for (int i = 0; i < p.stages; ++i) {
                 if (ok) {
-                    ok = mbar_wait(empty + 8 * stage, phase ^ 1, abort_flag, 2, limit);
+                    ok = mbar_wait_warp(empty + 8 * stage, phase ^ 1, abort_flag, 2, limit);
                 } else if (rank == 0) {
                     mbar_wait_drain(full + 8 * stage, phase ^ 1);
                 }
-                if (++stage == kPairStages) {
+                if (++stage == p.stages) {
                     stage = 0;
                     phase ^= 1;
                 }
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0 && !gave_up_before) {
+        if (rank == 0 && !gave_up_before) {
+            const bool one = elect_one();
             const uint32_t ring = smem_u32(smem);
             int stage = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
             bool ok = true;
             for (int t = pair; t < tiles && ok; t += pairs) {
-                if (!mbar_wait(acc_empty + 8 * acc, acc_phase ^ 1, abort_flag, 3, limit)) {
-                    ok = false;
-                    break;
-                }
+                ok = mbar_wait_warp(acc_empty + 8 * acc, acc_phase ^ 1, abort_flag, 3, limit);
+                if (!ok) break;
                 tc_fence_after();
                 const uint32_t d = tmem + acc * 256;
-                for (int ks = ks0; ks < ks1; ks += kSub) {
-                    if (!mbar_wait(full + 8 * stage, phase, abort_flag, 4, limit)) {
-                        ok = false;
-                        break;
-                    }
+                for (int ks = 0; ks < p.k_steps; ks += kSub) {
+                    ok = mbar_wait_warp(full + 8 * stage, phase, abort_flag, 4, limit);
+                    if (!ok) break;
                     tc_fence_after();
-                    const uint32_t a = desc_lo(ring + stage * kPairStageBytes, 16);
-                    const uint32_t b = desc_lo(ring + stage * kPairStageBytes + kRowTile, 16);
+                    const uint32_t a = desc_lo(ring + stage * kSub * step_bytes, 16);
+                    const uint32_t b = desc_lo(ring + stage * kSub * step_bytes + kRowTile, 16);
+                    if (one) {
 #pragma unroll
-                    for (int j = 0; j < kSub; ++j) {
-                        if (ks + j >= ks1) break;
+                        for (int j = 0; j < kSub; ++j) {
+                            if (ks + j >= p.k_steps) break;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)  // 32 bytes of k per MMA
-                            umma_ss_pair<kFp8>(d, a + j * (kPairStepBytes >> 4) + 2 * i, b + j * (kPairStepBytes >> 4) + 2 * i,
-                                               kDescHiSbo1024, p.idesc, ks > ks0 || (j | i) != 0);
+                            for (int i = 0; i < 4; ++i)  // 32 bytes of k per MMA
+                                umma_ss_pair<kFp8>(d, a + j * (step_bytes >> 4) + 2 * i, b + j * (step_bytes >> 4) + 2 * i,
+                                                   kDescHiSbo1024, p.idesc, (ks | j | i) != 0);
+                        }
+                        umma_commit_pair(empty + 8 * stage);
+                        if (ks + kSub >= p.k_steps) umma_commit_pair(acc_full + 8 * acc);
                     }
-                    umma_commit_pair(empty + 8 * stage, both_blocks);
-                    if (++stage == kPairStages) {
+                    __syncwarp();
+                    if (++stage == p.stages) {
                         stage = 0;
                         phase ^= 1;
                     }
                 }
-                if (ok) umma_commit_pair(acc_full + 8 * acc, both_blocks);
                 if ((acc ^= 1) == 0) acc_phase ^= 1;
             }
             if (!ok) {  // tensor memory and the operands stay until the MMAs that were issued are over
-                umma_commit_pair(drain, both_blocks);
+                if (one) umma_commit_pair(drain);
                 mbar_wait_drain(drain, 0);
             }
         }
@@ -425,7 +421,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
         char* buf = staging + (warp - 4) * kStagingBytes;
         constexpr int kCols = kMaxUnits * kUnit;
         float* cols = reinterpret_cast<float*>(columns + (warp - 4) * kColsBytes);  // [bias | weight scale | gate][kCols]
-        const uint32_t acc_empty0 = cluster_map(acc_empty, first);
+        const uint32_t acc_empty0 = cluster_map(acc_empty, 0);
         const uint16_t* residual = static_cast<const uint16_t*>(e.residual);
         uint4 ahead[2];  // the residual of the next unit
         int acc = 0;
@@ -528,107 +524,49 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
             };
             const uint32_t tmem_rows = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
             const float nan = __uint_as_float(0x7fc00000u);  // what a wait that gave up leaves: never plausible numbers
-            if constexpr (!kSplit) {
-                if (e.residual) fetch_unit(ahead, residual_at, tn * p.tile_n + turn * kUnit, e.n, e.wide_residual, lane);
-                // The first tile starts with a pass beyond the last column, which loads and stores nothing: it brings
-                // the code below into the instruction cache while the first MMAs run.
+            if (e.residual) fetch_unit(ahead, residual_at, tn * p.tile_n + turn * kUnit, e.n, e.wide_residual, lane);
+            // The first tile starts with a pass beyond the last column, which loads and stores nothing: it brings
+            // the code below into the instruction cache while the first MMAs run.
 #pragma unroll 1
-                for (int j = t == pair ? -1 : 0, u = turn + kUnitWarps * j; u < units; ++j, u += kUnitWarps) {
-                    const int col0 = j < 0 ? e.n : tn * p.tile_n + u * kUnit;
-                    if (j == 0) {
-                        if (ok) ok = mbar_wait(acc_full + 8 * acc, acc_phase, abort_flag, 5, limit);
-                        ok = __all_sync(0xffffffffu, ok);
-                        tc_fence_after();
-                    }
-                    uint64_t v[kUnit / 2];
-                    {
-                        uint32_t bits[16];
-                        if (ok && j >= 0) {
-                            tmem_ld16(tmem_rows + acc * 256 + u * kUnit, bits);
-                            tmem_wait_ld();
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < kUnit; ++i) bits[i] = __float_as_uint(nan);
-                        }
-#pragma unroll
-                        for (int i = 0; i < kUnit / 2; ++i) v[i] = pack2(__uint_as_float(bits[2 * i]), __uint_as_float(bits[2 * i + 1]));
-                    }
-                    if (col0 >= e.n && j >= 0) continue;
-                    if (e.residual && j >= 0) {
-                        put_unit(buf, ahead, lane);
-                        __syncwarp();
-                        if (u + kUnitWarps < units)
-                            fetch_unit(ahead, residual_at, col0 + kUnitWarps * kUnit, e.n, e.wide_residual, lane);
-                    }
-                    finish(v, j < 0 ? 0 : j, col0);
-                }
-                if (units <= turn) {  // a tile with fewer units than warps: this one only hands the accumulator back
+            for (int j = t == pair ? -1 : 0, u = turn + kUnitWarps * j; u < units; ++j, u += kUnitWarps) {
+                const int col0 = j < 0 ? e.n : tn * p.tile_n + u * kUnit;
+                if (j == 0) {
                     if (ok) ok = mbar_wait(acc_full + 8 * acc, acc_phase, abort_flag, 5, limit);
                     ok = __all_sync(0xffffffffu, ok);
+                    tc_fence_after();
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0 && ok) mbar_arrive_cluster(acc_empty0 + 8 * acc);
-                if ((acc ^= 1) == 0) acc_phase ^= 1;
-            } else {
-                // The ring is free once the accumulator is complete: it takes this pair's partial sums, in units of
-                // 128 rows x 64 bytes whose 16-byte pieces are permuted within a row against bank conflicts.  After
-                // a wait that gave up copies may still land there, so nothing is written; the flag speaks for it.
-                const int at = quarter * 32 + lane;
-                auto piece = [&](int u, int q) { return u * 8192 + at * 64 + ((q ^ ((at >> 1) & 3)) << 4); };
-                int failed = 0;
-                // Unit j of every warp is finished by pair j mod split, which adds the pairs' sums in their order.
-                // (j = -1: the pass that brings the code into the instruction cache.)
-#pragma unroll 1
-                for (int j = -1; j <= 0 || turn + kUnitWarps * j < units; ++j) {
-                    const int u = turn + kUnitWarps * j, col0 = j < 0 ? e.n : tn * p.tile_n + u * kUnit;
-                    if (j == 0) {
-                        if (ok) ok = mbar_wait(acc_full, 0, abort_flag, 5, limit);
-                        ok = __all_sync(0xffffffffu, ok);
-                        tc_fence_after();
-                        for (int w = turn; w < units && ok; w += kUnitWarps) {
-                            uint32_t bits[16];
-                            tmem_ld16(tmem_rows + w * kUnit, bits);
-                            tmem_wait_ld();
+                uint64_t v[kUnit / 2];
+                {
+                    uint32_t bits[16];
+                    if (ok && j >= 0) {
+                        tmem_ld16(tmem_rows + acc * 256 + u * kUnit, bits);
+                        tmem_wait_ld();
+                    } else {
 #pragma unroll
-                            for (int q = 0; q < 4; ++q)
-                                *reinterpret_cast<uint4*>(smem + piece(w, q)) =
-                                    make_uint4(bits[4 * q], bits[4 * q + 1], bits[4 * q + 2], bits[4 * q + 3]);
-                        }
-                        tc_fence_before();
-                        __syncwarp();
-                        cluster_sync_all();
-                        for (int i = 0; i < p.split; ++i) {
-                            failed |= cluster_load_i32(cluster_map(smem_u32(const_cast<int*>(abort_flag)), 2 * i + rank));
-                            failed |= cluster_load_i32(cluster_map(smem_u32(dead), 2 * i + rank));
-                        }
+                        for (int i = 0; i < kUnit; ++i) bits[i] = __float_as_uint(nan);
                     }
-                    if (j >= 0 && (u >= units || j % p.split != share || col0 >= e.n)) continue;
-                    if (e.residual) fetch_unit(ahead, residual_at, col0, e.n, e.wide_residual, lane);
-                    uint64_t v[kUnit / 2];
 #pragma unroll
-                    for (int i = 0; i < kUnit / 2; ++i) v[i] = both(failed ? nan : 0.0f);
-                    for (int i = 0; i < p.split && j >= 0; ++i) {
-                        float4 part[4];
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) part[q] = cluster_load_f32x4(cluster_map(smem_u32(smem) + piece(u, q), 2 * i + rank));
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            v[2 * q] = add2(v[2 * q], pack2(part[q].x, part[q].y));
-                            v[2 * q + 1] = add2(v[2 * q + 1], pack2(part[q].z, part[q].w));
-                        }
-                    }
-                    if (e.residual) {
-                        put_unit(buf, ahead, lane);
-                        __syncwarp();
-                    }
-                    finish(v, j < 0 ? 0 : j, col0);
+                    for (int i = 0; i < kUnit / 2; ++i) v[i] = pack2(__uint_as_float(bits[2 * i]), __uint_as_float(bits[2 * i + 1]));
                 }
+                if (col0 >= e.n && j >= 0) continue;
+                if (e.residual && j >= 0) {
+                    put_unit(buf, ahead, lane);
+                    __syncwarp();
+                    if (u + kUnitWarps < units)
+                        fetch_unit(ahead, residual_at, col0 + kUnitWarps * kUnit, e.n, e.wide_residual, lane);
+                }
+                finish(v, j < 0 ? 0 : j, col0);
             }
+            if (units <= turn) {  // a tile with fewer units than warps: this one only hands the accumulator back
+                if (ok) ok = mbar_wait(acc_full + 8 * acc, acc_phase, abort_flag, 5, limit);
+                ok = __all_sync(0xffffffffu, ok);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0 && ok) mbar_arrive_cluster(acc_empty0 + 8 * acc);
+            if ((acc ^= 1) == 0) acc_phase ^= 1;
         }
     }
-    __syncwarp();
-    if (kSplit && warp < 4) cluster_sync_all();  // the one between the partial sums and their addition
     __syncwarp();
     tc_fence_before();
     __syncthreads();
@@ -641,15 +579,15 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
 // ---- few rows ----------------------------------------------------------------------------------------------
 
 constexpr int kSwapThreads = 192;  // warps: 0 loader, 1 tensor memory + MMA, 2..5 epilogue
-constexpr int kSwapMaxStages = 16;
+constexpr int kSwapMaxStages = 8;
 constexpr int kSwapCtlBytes = 16 * kSwapMaxStages + 64;
 
 template <bool kFp8>
 __global__ void __launch_bounds__(kSwapThreads) linear_swap_kernel(const __grid_constant__ LinearParams p) {
     extern __shared__ char smem_raw[];
     char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    const uint32_t stage_bytes = kRowTile + static_cast<uint32_t>(p.tile_n) * kStepBytes;
-    char* ctl = smem + p.stages * stage_bytes;
+    const uint32_t step_bytes = kRowTile + static_cast<uint32_t>(p.tile_n) * kStepBytes;
+    char* ctl = smem + p.stages * kSub * step_bytes;
     const uint32_t full = smem_u32(ctl), empty = full + 8 * kSwapMaxStages, done = empty + 8 * kSwapMaxStages;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctl + 16 * kSwapMaxStages + 8);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -728,19 +666,23 @@ __global__ void __launch_bounds__(kSwapThreads) linear_swap_kernel(const __grid_
     }
 
     if (warp == 0) {
-        if (lane == 0 && ok && !p.test_withhold) {
+        if (ok && !p.test_withhold) {
+            const bool one = elect_one();
             const uint32_t ring = smem_u32(smem);
             int stage = 0;
             uint32_t phase = 0;
-            for (int ks = ks0; ks < ks1; ++ks) {
-                if (!mbar_wait(empty + 8 * stage, phase ^ 1, abort_flag, 6, limit)) {
-                    ok = false;
-                    break;
+            for (int ks = ks0; ks < ks1; ks += kSub) {
+                ok = mbar_wait_warp(empty + 8 * stage, phase ^ 1, abort_flag, 6, limit);
+                if (!ok) break;
+                const int subs = min(kSub, ks1 - ks);
+                if (one) {
+                    mbar_arrive_expect_tx(full + 8 * stage, subs * step_bytes);
+                    uint32_t dst = ring + stage * kSub * step_bytes;
+                    for (int j = 0; j < subs; ++j, dst += step_bytes) {
+                        tma_load_4d(dst, &p.tm_w, full + 8 * stage, (ks + j) * p.k_step_elems, row_w, 0, 0);
+                        tma_load_4d(dst + kRowTile, &p.tm_x, full + 8 * stage, (ks + j) * p.k_step_elems, row_x, 0, 0);
+                    }
                 }
-                mbar_arrive_expect_tx(full + 8 * stage, stage_bytes);
-                const uint32_t dst = ring + stage * stage_bytes;
-                tma_load_4d(dst, &p.tm_w, full + 8 * stage, ks * p.k_step_elems, row_w, 0, 0);
-                tma_load_4d(dst + kRowTile, &p.tm_x, full + 8 * stage, ks * p.k_step_elems, row_x, 0, 0);
                 if (++stage == p.stages) {
                     stage = 0;
                     phase ^= 1;
@@ -756,25 +698,34 @@ __global__ void __launch_bounds__(kSwapThreads) linear_swap_kernel(const __grid_
                 }
         }
     } else if (warp == 1) {
-        if (lane == 0 && ok) {
+        if (ok) {
+            const bool one = elect_one();
             const uint32_t ring = smem_u32(smem);
             int stage = 0;
             uint32_t phase = 0;
-            for (int ks = ks0; ks < ks1; ++ks) {
-                if (!mbar_wait(full + 8 * stage, phase, abort_flag, 7, limit)) break;
+            for (int ks = ks0; ks < ks1; ks += kSub) {
+                if (!mbar_wait_warp(full + 8 * stage, phase, abort_flag, 7, limit)) break;
                 tc_fence_after();
-                const uint32_t a = desc_lo(ring + stage * stage_bytes, 16);
-                const uint32_t b = desc_lo(ring + stage * stage_bytes + kRowTile, 16);
+                const uint32_t a = desc_lo(ring + stage * kSub * step_bytes, 16);
+                const uint32_t b = desc_lo(ring + stage * kSub * step_bytes + kRowTile, 16);
+                if (one) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    umma_ss_lohi<kFp8>(tmem, a + 2 * i, b + 2 * i, kDescHiSbo1024, p.idesc, (ks > ks0 || i) ? 1u : 0u);
-                umma_commit(empty + 8 * stage);
+                    for (int j = 0; j < kSub; ++j) {
+                        if (ks + j >= ks1) break;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            umma_ss_lohi<kFp8>(tmem, a + j * (step_bytes >> 4) + 2 * i, b + j * (step_bytes >> 4) + 2 * i,
+                                               kDescHiSbo1024, p.idesc, ks > ks0 || (j | i) != 0);
+                    }
+                    umma_commit(empty + 8 * stage);
+                }
+                __syncwarp();
                 if (++stage == p.stages) {
                     stage = 0;
                     phase ^= 1;
                 }
             }
-            umma_commit(done);  // also after a wait that gave up: the MMAs that were issued must be over
+            if (one) umma_commit(done);  // also after a wait that gave up: the MMAs that were issued must be over
             mbar_wait_drain(done, 0);
         }
     }
@@ -871,41 +822,44 @@ cudaError_t launch_clusters(Kernel kernel, const LinearParams& p, dim3 grid, int
 template <bool kFp8>
 cudaError_t launch_pair(const LinearParams& p, cudaStream_t stream) {
     const int tiles = p.tiles_m * p.tiles_n;
-    if (p.split > 1)
-        return launch_clusters(linear_pair_kernel<kFp8, true>, p, dim3(2 * p.split * tiles), 2 * p.split, kPairThreads, kPairSmem, stream);
-    return launch_clusters(linear_pair_kernel<kFp8, false>, p, dim3(2 * (tiles < kSms / 2 ? tiles : kSms / 2)), 2, kPairThreads,
-                           kPairSmem, stream);
+    const dim3 grid(2 * (tiles < kSms / 2 ? tiles : kSms / 2));
+    return launch_clusters(linear_pair_kernel<kFp8>, p, grid, 2, kPairThreads, kPairSmem, stream);
 }
 
 // How a product is cut up.
 struct Plan {
     bool swap;
     int tile_n;         // pair: columns, swap: tokens
-    int stages;         // swap
-    int split;          // blocks (swap) or pairs (pair) that share the k of a tile
+    int stages;
+    int split;          // swap: blocks of a cluster that share the k of a tile
     int band;           // pair
 };
 
 constexpr int swap_columns(int tile_n) { return tile_n <= 32 ? 32 : tile_n <= 64 ? 64 : tile_n <= 128 ? 128 : 256; }
-constexpr int swap_smem(int tile_n, int stages) { return stages * (kRowTile + tile_n * kStepBytes) + kSwapCtlBytes + 1024; }
+constexpr int swap_smem(int tile_n, int stages) { return stages * kSub * (kRowTile + tile_n * kStepBytes) + kSwapCtlBytes + 1024; }
+
+constexpr int pair_stages(int tile_n) {
+    const int stages = kRingBytes / (kSub * (kRowTile + tile_n / 2 * kStepBytes));
+    return stages < kPairMaxStages ? stages : kPairMaxStages;
+}
 
 Plan choose_plan(int m, int n, int k_steps) {
     Plan plan = {};
     if (m <= 128) {
         plan.swap = true;
         plan.tile_n = (m + 15) / 16 * 16;
-        const int stage_bytes = kRowTile + plan.tile_n * kStepBytes;
-        plan.stages = (74 * 1024 - swap_smem(0, 0)) / stage_bytes;
-        if (plan.stages < 4) plan.stages = 4;
+        const int stage_bytes = kSub * (kRowTile + plan.tile_n * kStepBytes);
+        plan.stages = (112 * 1024 - swap_smem(0, 0)) / stage_bytes;
+        if (plan.stages < 2) plan.stages = 2;
         const int blocks = (n + 127) / 128;
         const int slots = kSms * (kMaxSmem / (swap_smem(plan.tile_n, plan.stages) + 1024));
         plan.split = 1;
-        while (plan.split < 8 && (plan.split + 1) * blocks <= slots && k_steps >= 2 * (plan.split + 1)) ++plan.split;
+        while (plan.split < 8 && (plan.split + 1) * blocks <= slots && k_steps >= 2 * kSub * (plan.split + 1)) ++plan.split;
     } else {
         plan.tile_n = 256;
         plan.band = 8;
-        plan.split = 1;
     }
+    if (!plan.swap) plan.stages = pair_stages(plan.tile_n);
     return plan;
 }
 
@@ -984,10 +938,10 @@ extern "C" int mindiesd_linear_fwd(const mindiesd_linear_args* a, void* stream_)
     const Plan plan = choose_plan(a->m, a->n, p.k_steps);
     p.tile_n = plan.tile_n;
     p.split = plan.split;
+    p.stages = plan.stages;
     if (plan.swap) {
         p.tmem_cols = swap_columns(p.tile_n);
         p.idesc = umma_idesc(fmt, 128, p.tile_n, false, false);
-        p.stages = plan.stages;
         if ((a->n + 127) / 128 > 65535 || (a->m + p.tile_n - 1) / p.tile_n > 65535) return MINDIESD_E_CAPACITY;
         if ((rc = encode_tile_map(&p.tm_w, a->weight, a->in_dtype, a->k, a->n, 1, 1, w_strides, 128))) return rc;
         if ((rc = encode_tile_map(&p.tm_x, a->x, a->in_dtype, a->k, a->m, 1, 1, x_strides, p.tile_n))) return rc;

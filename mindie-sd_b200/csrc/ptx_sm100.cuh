@@ -75,6 +75,32 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     return false;
 }
 
+// The same wait by a whole warp, with one answer for all lanes.  A loop whose control flow is uniform keeps its
+// addresses and descriptors in uniform registers; one that runs in a single lane's branch pays for moving each of
+// them there in front of every copy and every MMA.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int site,
+                                               uint32_t limit_us) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    const uint64_t t0 = global_timer_ns();
+    for (uint32_t i = 1;; ++i) {
+        if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+        if ((i & 63u) == 0u) {
+            const bool late = global_timer_ns() - t0 > static_cast<uint64_t>(limit_us) * 1000u;
+            if (__any_sync(0xffffffffu, *abort_flag != 0 || late)) break;
+        }
+    }
+    if (*abort_flag == 0) abort_flag[1] = site;
+    *abort_flag = 1;
+    return false;
+}
+
+// True in one lane of the warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+
 // The wait of a thread that must see its own asynchronous copies land before the thread block may
 // exit: it does not look at the abort flag (the copies are in flight whatever the other roles
 // decided) and is bounded by time alone.
@@ -293,12 +319,11 @@ __device__ __forceinline__ void umma_ss_pair(uint32_t d_tmem, uint32_t a_lo, uin
             : "memory");
     }
 }
-// One arrival on the barrier at this offset in the blocks of the cluster that `blocks` names (both of the pair),
-// once every MMA issued so far is complete.
-__device__ __forceinline__ void umma_commit_pair(uint32_t bar, uint16_t blocks) {
+// One arrival on the barrier at this offset in BOTH blocks of the pair, once every MMA issued so far is complete.
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
     asm volatile(
         "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-        "h"(blocks)
+        "h"(static_cast<uint16_t>(3))
         : "memory");
 }
 // Shared-memory matrix descriptor of a 128-byte-swizzled operand tile, as low and high word.
