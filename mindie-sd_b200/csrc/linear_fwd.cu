@@ -18,6 +18,10 @@
 #include "ptx_sm100.cuh"
 #include "row_io.cuh"
 
+#include <algorithm>
+#include <atomic>
+#include <mutex>
+
 namespace sdb {
 namespace {
 
@@ -800,73 +804,189 @@ __global__ void __launch_bounds__(kSwapThreads) linear_swap_kernel(const __grid_
 constexpr int kSms = 148;
 constexpr int kMaxSmem = 227 * 1024;
 
-template <typename Kernel>
-cudaError_t launch_clusters(Kernel kernel, const LinearParams& p, dim3 grid, int cluster, int threads, int smem, cudaStream_t stream) {
-    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (err != cudaSuccess) return err;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads, 1, 1);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
+// A launch configuration whose clusters span the x dimension.
+struct ClusterLaunch {
     cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, p);
+    cudaLaunchConfig_t cfg = {};
+    ClusterLaunch(dim3 grid, int cluster, int threads, int smem, cudaStream_t stream) {
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = cluster;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.gridDim = grid;
+        cfg.blockDim = dim3(threads, 1, 1);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = stream;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+    }
+};
+
+// Lets a kernel use all of an SM's shared memory, once per device (a call that set the limit to its own need could
+// lower it under another thread's launch).
+template <auto kKernel>
+cudaError_t allow_all_shared_memory() {
+    constexpr int kMaxDevices = 64;
+    static std::atomic<bool> done[kMaxDevices];
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
+    if (err != cudaSuccess || (dev < kMaxDevices && done[dev].load(std::memory_order_acquire))) return err;
+    err = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+    if (err == cudaSuccess && dev < kMaxDevices) done[dev].store(true, std::memory_order_release);
+    return err;
+}
+
+template <auto kKernel>
+cudaError_t launch_clusters(const LinearParams& p, dim3 grid, int cluster, int threads, int smem, cudaStream_t stream) {
+    const cudaError_t err = allow_all_shared_memory<kKernel>();
+    if (err != cudaSuccess) return err;
+    ClusterLaunch launch(grid, cluster, threads, smem, stream);
+    return cudaLaunchKernelEx(&launch.cfg, kKernel, p);
 }
 
 template <bool kFp8>
 cudaError_t launch_pair(const LinearParams& p, cudaStream_t stream) {
     const int tiles = p.tiles_m * p.tiles_n;
     const dim3 grid(2 * (tiles < kSms / 2 ? tiles : kSms / 2));
-    return launch_clusters(linear_pair_kernel<kFp8>, p, grid, 2, kPairThreads, kPairSmem, stream);
+    return launch_clusters<linear_pair_kernel<kFp8>>(p, grid, 2, kPairThreads, kPairSmem, stream);
 }
 
 // How a product is cut up.
 struct Plan {
     bool swap;
-    int tile_n;         // pair: columns, swap: tokens
+    int tile_n;  // pair: columns, swap: tokens
     int stages;
-    int split;          // swap: blocks of a cluster that share the k of a tile
-    int band;           // pair
+    int split;   // swap: blocks of a cluster that share the k of a tile
+    int band;    // pair
 };
 
-constexpr int swap_columns(int tile_n) { return tile_n <= 32 ? 32 : tile_n <= 64 ? 64 : tile_n <= 128 ? 128 : 256; }
+constexpr int swap_columns(int tile_n) { return tile_n <= 32 ? 32 : tile_n <= 64 ? 64 : 128; }
 constexpr int swap_smem(int tile_n, int stages) { return stages * kSub * (kRowTile + tile_n * kStepBytes) + kSwapCtlBytes + 1024; }
+constexpr int kSwapMaxTile = 128, kSwapMaxSplit = 8;
 
+// Stages that let `per_sm` blocks of the swap kernel share an SM (1 KB of each goes to the system).  Blocks that fit
+// by their shared memory also fit by their tensor memory (at most 2 x 128 columns of 512), so an allocation of
+// one never waits for another block of its kind.
+constexpr int swap_stages(int tile_n, int per_sm) {
+    const int stages = (228 * 1024 / per_sm - 1024 - swap_smem(0, 0)) / (kSub * (kRowTile + tile_n * kStepBytes));
+    return stages < kSwapMaxStages ? stages : kSwapMaxStages;
+}
 constexpr int pair_stages(int tile_n) {
     const int stages = kRingBytes / (kSub * (kRowTile + tile_n / 2 * kStepBytes));
     return stages < kPairMaxStages ? stages : kPairMaxStages;
 }
 
-Plan choose_plan(int m, int n, int k_steps) {
-    Plan plan = {};
-    if (m <= 128) {
-        plan.swap = true;
-        plan.tile_n = (m + 15) / 16 * 16;
-        const int stage_bytes = kSub * (kRowTile + plan.tile_n * kStepBytes);
-        plan.stages = (112 * 1024 - swap_smem(0, 0)) / stage_bytes;
-        if (plan.stages < 2) plan.stages = 2;
-        const int blocks = (n + 127) / 128;
-        const int slots = kSms * (kMaxSmem / (swap_smem(plan.tile_n, plan.stages) + 1024));
-        plan.split = 1;
-        while (plan.split < 8 && (plan.split + 1) * blocks <= slots && k_steps >= 2 * kSub * (plan.split + 1)) ++plan.split;
-    } else {
-        plan.tile_n = 256;
-        plan.band = 8;
+// Clusters of 1..8 blocks that the device holds at once with one and with two blocks per SM.  A cluster lies inside
+// one group of SMs, so these are not 148 / size: measured 15 of eight blocks, not 18, and a 16th one is a second wave.
+struct Residency {
+    int clusters[2][kSwapMaxSplit + 1];
+};
+const Residency& residency() {
+    constexpr int kMaxDevices = 64;
+    static std::mutex mu;
+    static Residency table[kMaxDevices];
+    static bool known[kMaxDevices] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) dev = 0;
+    std::lock_guard<std::mutex> lock(mu);
+    Residency& r = table[dev];
+    if (!known[dev]) {
+        allow_all_shared_memory<linear_swap_kernel<false>>();
+        for (int per_sm = 1; per_sm <= 2; ++per_sm) {
+            const int smem = swap_smem(16, swap_stages(16, per_sm));
+            for (int size = 1; size <= kSwapMaxSplit; ++size) {
+                ClusterLaunch launch(dim3(size), size, kSwapThreads, smem, nullptr);
+                int n = 0;
+                if (cudaOccupancyMaxActiveClusters(&n, linear_swap_kernel<false>, &launch.cfg) != cudaSuccess || n <= 0) {
+                    cudaGetLastError();
+                    n = kSms * per_sm / size;
+                }
+                r.clusters[per_sm - 1][size] = n;
+            }
+        }
+        known[dev] = true;
     }
-    if (!plan.swap) plan.stages = pair_stages(plan.tile_n);
-    return plan;
+    return r;
+}
+
+// The plan with the smallest estimated time.  The estimates are a model of the two kernels (microseconds) whose
+// constants were fitted to 12 900 timings of 300 products (m 1..16000, k 64..20480, n 16..20480, both operand
+// widths, operands in HBM): the plan it picks is 1.2 % slower than the best measured one on average, and more
+// than 10 % slower for 17 of the 300.  What it weighs, with both sides measured (bf16, k 5120, n 5120):
+//   m 64:   swap, 3 blocks per tile 16.0 us, 8 blocks 23 us (clusters of a second wave); pair 21.3 us
+//   m 256:  pair, 96 columns (54 tiles) 21.3 us, 256 columns (20 tiles) 32 us; swap 26.3 us
+//   m 2048: pair, 192 columns (216 tiles, 2.92 waves) 78 us, 256 columns (160 tiles, 2.16 waves) 94 us
+Plan estimate_plan(int m, int n, int k_steps) {
+    auto ceil_div = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
+    const double bytes = (static_cast<double>(m) + n) * k_steps * kStepBytes + 2.0 * m * n;
+    // The larger of the two times, and a share of the smaller one that the other does not hide.
+    auto overlap = [](double busy, double memory, double share) { return std::max(busy, memory) + share * std::min(busy, memory); };
+    constexpr double kMemory = 5.38e6, kMemoryOfBlock = 60e3;  // bytes per microsecond: 5.38 TB/s, 60 GB/s for one block
+    Plan best = {};
+    double best_us = 1e300;
+    for (int tile_n = 32; tile_n <= 256; tile_n += 32) {
+        if (tile_n > ceil_div(n, 32) * 32) break;
+        const int64_t tiles = ceil_div(m, 256) * ceil_div(n, tile_n);
+        const double waves = static_cast<double>(ceil_div(tiles, kSms / 2));
+        // A k step of a tile: its MMAs, the round trip of its barriers, or the pairs' loads from L2 at 22.8 TB/s.
+        double step = std::max(0.199, 0.00117 * tile_n);
+        step = std::max(step, static_cast<double>(std::min<int64_t>(tiles, kSms / 2)) * 2 * (kRowTile + tile_n * 64) / 22.8e6);
+        const double units = static_cast<double>(ceil_div(tile_n / kUnit, kUnitWarps));
+        const double us = 3.28 + overlap(waves * std::max(k_steps * step, units), bytes / kMemory, 0.127) + 0.236 * units + 1.16 * waves;
+        if (us < best_us) {
+            best_us = us;
+            best = {false, tile_n, pair_stages(tile_n), 1, 8};
+        }
+    }
+    const int64_t blocks_n = ceil_div(n, 128);
+    int last = 0;
+    for (int want = 16; want <= kSwapMaxTile; want += 16) {
+        const int64_t parts = ceil_div(m, want);
+        if (blocks_n * parts > 2 * kSms * 2) continue;
+        const int tile = static_cast<int>(ceil_div(ceil_div(m, parts), 16) * 16);  // even parts
+        if (tile == last) continue;
+        last = tile;
+        for (int per_sm = 1; per_sm <= 2; ++per_sm) {
+            const int stages = swap_stages(tile, per_sm);
+            if (stages < 2) continue;
+            for (int split = 1; split <= kSwapMaxSplit && (split == 1 || k_steps >= 2 * split); ++split) {
+                const int64_t clusters = blocks_n * parts, room = residency().clusters[per_sm - 1][split];
+                const double waves = static_cast<double>(ceil_div(clusters, room));
+                const double active = static_cast<double>(std::min(clusters, room)) * split;
+                double step = std::max(0.219, 0.0033 * tile) * (1 + 0.69 * (std::max(1.0, active / kSms) - 1));
+                step = std::max(step, active * (kRowTile + tile * kStepBytes) / 9.6e6);
+                const double reduce = 0.076 * std::min(tile, m) / split + (split > 1 ? 1.04 : 0.0);
+                const double steps = static_cast<double>(ceil_div(ceil_div(k_steps, split), kSub) * kSub);
+                const double us = 2.66 + overlap(waves * steps * step, bytes / std::min(kMemory, active * kMemoryOfBlock), 0.089) + reduce * waves + 1.23 * (waves - 1);
+                if (us < best_us) {
+                    best_us = us;
+                    best = {true, tile, stages, split, 0};
+                }
+            }
+        }
+    }
+    return best;
+}
+
+// The plan depends on the sizes alone, so the estimates (2 us of host time) are made once for each.
+Plan choose_plan(int m, int n, int k_steps) {
+    struct Entry {
+        int m, n, k_steps;
+        Plan plan;
+    };
+    constexpr int kEntries = 64;
+    thread_local Entry cache[kEntries] = {};
+    const unsigned h = (static_cast<unsigned>(m) * 0x9e3779b1u) ^ (static_cast<unsigned>(n) * 0x85ebca6bu) ^
+                       (static_cast<unsigned>(k_steps) * 0xc2b2ae35u);
+    Entry& c = cache[(h ^ (h >> 15)) % kEntries];
+    if (c.m != m || c.n != n || c.k_steps != k_steps) c = {m, n, k_steps, estimate_plan(m, n, k_steps)};
+    return c.plan;
 }
 
 template <bool kFp8>
 cudaError_t launch_swap(const LinearParams& p, cudaStream_t stream) {
     const dim3 grid(p.split, (p.e.n + 127) / 128, (p.e.m + p.tile_n - 1) / p.tile_n);
-    return launch_clusters(linear_swap_kernel<kFp8>, p, grid, p.split, kSwapThreads, swap_smem(p.tile_n, p.stages), stream);
+    return launch_clusters<linear_swap_kernel<kFp8>>(p, grid, p.split, kSwapThreads, swap_smem(p.tile_n, p.stages), stream);
 }
 
 }  // namespace
