@@ -59,6 +59,16 @@ struct Run {
     __device__ __forceinline__ void set(int i, float v) { d.elem[i] = from_f32<T>(v); }
 };
 
+__device__ __forceinline__ uint4 load_shared16(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ void store_shared16(uint32_t addr, const uint4& v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
 // Maximum that keeps a NaN (fmaxf drops it).
 __device__ __forceinline__ float max_nan(float a, float b) {
     float d;

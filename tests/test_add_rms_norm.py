@@ -157,6 +157,39 @@ def test_token_quant(dim, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim", [8, 64, 128, 200, 1000, 1536, 5120, 10240, 16384, 24576])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_many_rows(dim, dtype):
+    """Enough rows that the blocks of the launch walk several each, ragged at the end; every row is looked at."""
+    from mindiesd import add_rms_norm, add_rms_norm_quant
+    rows = {8: 200001, 64: 70003, 128: 40005, 200: 30001}.get(dim, 2503)
+    for weight, residual in [(None, None), (dtype, dtype), (torch.float32, torch.float32)]:
+        x = _randn(dim, rows, dim, dtype=dtype)
+        w = None if weight is None else _randn(1, dim, dtype=weight)
+        r = None if residual is None else _randn(2, rows, dim, dtype=residual, scale=3.0)
+        y64, v64 = ob.rms_norm(x, w, r)
+        got, quant = add_rms_norm(x, w, r), add_rms_norm_quant(x, w, r)
+        if r is not None:
+            got, total = got
+            assert torch.equal(quant[2], total)
+            _close(total, v64, residual)
+        _close(got, y64, dtype)
+        _close_quant(quant[0], quant[1], y64)
+
+
+@pytest.mark.gpu
+def test_many_strided_rows():
+    from mindiesd import add_rms_norm
+    packed = _randn(3, 6000, 3 * 1536, dtype=torch.bfloat16)
+    weight = _randn(4, 1536, dtype=torch.bfloat16)
+    for part in (packed[:, :1536], packed.narrow(1, 1536, 1536), packed[:1, :1536].expand(6000, 1536)):
+        y, total = add_rms_norm(part, weight, packed[:, -1536:])
+        y64, v64 = ob.rms_norm(part, weight, packed[:, -1536:])
+        _close(y, y64, torch.bfloat16)
+        _close(total, v64, torch.bfloat16)
+
+
+@pytest.mark.gpu
 def test_long_rows():
     from mindiesd import add_rms_norm, add_rms_norm_quant
     for dim, dtype in ((70001, torch.bfloat16), (70000, torch.float32), (6145, torch.float16)):
