@@ -115,8 +115,7 @@ __device__ __forceinline__ void weights_of(const NormParams& p, int at, float (&
     }
 }
 
-// One row per `group` threads, kV runs of kE elements per thread, the row in registers.  Runs of 16 bytes
-// where every row starts on such a boundary, 8 bytes or single elements where only that holds.
+// Few rows that start on 16-byte boundaries: one row per `group` threads, kV runs of 16 bytes per thread.
 template <typename T, int kE, int kV>
 __global__ void __launch_bounds__(1024) norm_row_kernel(const NormParams p) {
     const int lane = threadIdx.x & (p.group - 1);
@@ -412,6 +411,81 @@ __global__ void __launch_bounds__(kRes > 0 ? 512 : 768) norm_stream_kernel(const
     }
 }
 
+// Rows that no 16-byte run fits: runs of four elements or single ones, straight from global memory, by blocks that
+// stay.  A thread has the next row's runs on their way in registers while it works on the present row, and takes 16
+// elements of it, because a row's reduction costs every thread the same whatever its share (20000 x 1001 bf16: a
+// block of 256 threads per row, four elements each, issued 75 instructions per element and took 64 us).  kRes: 0 no residual, 1 in the type of x, 2 fp32.
+template <typename T, int kE, int kV, int kRes>
+__global__ void __launch_bounds__(512) norm_narrow_kernel(const NormParams p) {
+    using R = std::conditional_t<kRes == 2, float, T>;
+    const int lane = threadIdx.x & (p.group - 1);
+    const int per_block = blockDim.x / p.group;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * per_block;
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * per_block + threadIdx.x / p.group;
+    Run<T, kE> in[kV];
+    Run<R, kE> add[kV];
+    auto fetch = [&](int64_t row) {
+        const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
+        const R* r = static_cast<const R*>(p.residual) + row * p.residual_stride;
+#pragma unroll
+        for (int j = 0; j < kV; ++j) {
+            const int at = (lane + j * p.group) * kE;
+            if (row >= p.rows || at >= p.dim) continue;
+            in[j].load(x + at);
+            if constexpr (kRes > 0) add[j].load(r + at);
+        }
+    };
+    fetch(first);
+    float w[kV][kE];  // a load of them within the loop would have to wait for the next row's runs as well
+#pragma unroll
+    for (int j = 0; j < kV; ++j) {
+        const int at = (lane + j * p.group) * kE;
+        if (at < p.dim) weights_of<T, kE>(p, at, w[j]);
+    }
+    int turn = 0;
+    for (int64_t row = first; row - threadIdx.x / p.group < p.rows; row += step) {
+        const bool live = row < p.rows;
+        float v[kV][kE];
+#pragma unroll
+        for (int j = 0; j < kV; ++j)
+#pragma unroll
+            for (int i = 0; i < kE; ++i) v[j][i] = kRes > 0 ? in[j].get(i) + add[j].get(i) : in[j].get(i);
+        fetch(row + step);
+        Stats s = {0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < kV; ++j) {
+            const int at = (lane + j * p.group) * kE;
+            if (!live || at >= p.dim) continue;
+            if constexpr (kRes > 0) {
+                Run<R, kE> r;
+#pragma unroll
+                for (int i = 0; i < kE; ++i) r.set(i, v[j][i]);
+                r.store(static_cast<R*>(p.residual_out) + row * p.dim + at);
+            }
+#pragma unroll
+            for (int i = 0; i < kE; ++i) {
+                s.sum += v[j][i] * v[j][i];
+                v[j][i] *= w[j][i];
+                if (p.scales) s.top = max_nan(s.top, fabsf(v[j][i]));
+            }
+        }
+        s = p.scales ? reduce_row<true>(s, p.group, turn) : reduce_row<false>(s, p.group, turn);
+        turn ^= 1;
+        float scale = 1.0f;
+        const float f = row_factor(p, s, scale);
+        if (!live) continue;
+        if (p.scales && lane == 0) p.scales[row] = scale;
+#pragma unroll
+        for (int j = 0; j < kV; ++j) {
+            const int at = (lane + j * p.group) * kE;
+            if (at >= p.dim) continue;
+#pragma unroll
+            for (int i = 0; i < kE; ++i) v[j][i] *= f;
+            store_run<T, kE>(p, row * p.dim + at, v[j]);
+        }
+    }
+}
+
 // Rows too long for the registers of a block: one block per row, the row read twice (the second time from L2).
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_long_kernel(const NormParams p) {
@@ -451,7 +525,6 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const NormParams p) {
 }
 
 constexpr int kSms = 148;
-constexpr int kMaxRuns = 6;  // of one thread in one row
 constexpr int kStreamBlocks = 4 * kSms;
 
 constexpr int kMaxSmem = 226 * 1024;  // of 227 KB, beside the partials of the reduction
@@ -489,51 +562,75 @@ cudaError_t launch_stream(const NormParams& p, int threads, cudaStream_t stream)
                     : launch_stream_as<T, kE, kV, kRes, false>(p, threads, stream);
 }
 
-template <typename T, int kE, int kV>
-cudaError_t launch_runs(const NormParams& p, int threads, cudaStream_t stream) {
+// Rows of 16-byte runs.
+template <typename T, int kV>
+cudaError_t launch_wide(const NormParams& p, int threads, cudaStream_t stream) {
+    constexpr int kE = 16 / sizeof(T);
     const int64_t blocks = (p.rows + threads / p.group - 1) / (threads / p.group);
-    if constexpr (kE * sizeof(T) == 16) {
-        // Worth its longer start only where a block walks several rows: 2000 rows of 5120 bf16 with a residual 15.6 us
-        // (norm_row_kernel 17.4), 300 rows as fast either way.
-        if (blocks > kStreamBlocks && threads <= 512) {
-            if (!p.residual) {
-                if (stream_smem<kV, 0>(threads) <= kMaxSmem) return launch_stream<T, kE, kV, 0>(p, threads, stream);
-            } else if (p.residual_fp32) {
-                if (stream_smem<kV, 4 * kE>(threads) <= kMaxSmem) return launch_stream<T, kE, kV, 4 * kE>(p, threads, stream);
-            } else {
-                if (stream_smem<kV, 16>(threads) <= kMaxSmem) return launch_stream<T, kE, kV, 16>(p, threads, stream);
-            }
+    // Worth its longer start only where a block walks several rows: 2000 rows of 5120 bf16 with a residual 15.6 us
+    // (norm_row_kernel 17.4), 300 rows as fast either way.
+    if (blocks > kStreamBlocks && threads <= 512) {
+        if (!p.residual) {
+            if (stream_smem<kV, 0>(threads) <= kMaxSmem) return launch_stream<T, kE, kV, 0>(p, threads, stream);
+        } else if (p.residual_fp32) {
+            if (stream_smem<kV, 4 * kE>(threads) <= kMaxSmem) return launch_stream<T, kE, kV, 4 * kE>(p, threads, stream);
+        } else {
+            if (stream_smem<kV, 16>(threads) <= kMaxSmem) return launch_stream<T, kE, kV, 16>(p, threads, stream);
         }
     }
     norm_row_kernel<T, kE, kV><<<static_cast<unsigned>(blocks), threads, 0, stream>>>(p);
     return cudaGetLastError();
 }
 
+template <typename T, int kE, int kV>
+cudaError_t launch_narrow(const NormParams& p, int threads, cudaStream_t stream) {
+    const int64_t blocks = (p.rows + threads / p.group - 1) / (threads / p.group);
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(blocks, kSms * (1024 / threads)));
+    if (!p.residual) norm_narrow_kernel<T, kE, kV, 0><<<grid, threads, 0, stream>>>(p);
+    else if (!p.residual_fp32) norm_narrow_kernel<T, kE, kV, 1><<<grid, threads, 0, stream>>>(p);
+    else norm_narrow_kernel<T, kE, kV, 2><<<grid, threads, 0, stream>>>(p);
+    return cudaGetLastError();
+}
+
 template <typename T, int kE>
 cudaError_t launch_rows(NormParams p, cudaStream_t stream) {
     const int runs = (p.dim + kE - 1) / kE;
+    constexpr bool kWide = kE * sizeof(T) == 16;
     // The smallest group of threads that holds the row in so many runs each: three 16-byte runs (75600 x 5120 bf16
     // with a residual 471 us, with six runs 490; 300 rows 4.5 us, six 5.7), six where the row is wide and has no
-    // residual (quantised 238 us, three 311: the reduction over twice the warps costs more than the loads) and six
-    // narrower runs (20000 x 1001 bf16 64 us, three 102).
-    const int most = kE * sizeof(T) == 16 && (p.residual || runs <= 384) ? 3 : kMaxRuns;
+    // residual (quantised 238 us, three 311: the reduction over twice the warps costs more than the loads).
+    const int most = !kWide ? 16 / kE : p.residual || runs <= 384 ? 3 : 6;
     int group = 1;
-    while (group < 1024 && group * most < runs) group *= 2;
-    const int per_thread = (runs + group - 1) / group;
-    if (per_thread > kMaxRuns) {
+    while (group < 512 && group * most < runs) group *= 2;
+    int per_thread = (runs + group - 1) / group;
+    if (kWide && per_thread > most) {
+        group = 1024;
+        per_thread = (runs + group - 1) / group;
+    }
+    if (per_thread > (kWide ? 6 : most)) {
         p.group = 1024;
         norm_long_kernel<T><<<static_cast<unsigned>(p.rows), 1024, 0, stream>>>(p);
         return cudaGetLastError();
     }
     p.group = group;
     const int threads = group > 128 ? group : 128;
-    switch (per_thread) {
-        case 1: return launch_runs<T, kE, 1>(p, threads, stream);
-        case 2: return launch_runs<T, kE, 2>(p, threads, stream);
-        case 3: return launch_runs<T, kE, 3>(p, threads, stream);
-        case 4: return launch_runs<T, kE, 4>(p, threads, stream);
-        case 5: return launch_runs<T, kE, 5>(p, threads, stream);
-        default: return launch_runs<T, kE, 6>(p, threads, stream);
+    if constexpr (kWide) {
+        switch (per_thread) {
+            case 1: return launch_wide<T, 1>(p, threads, stream);
+            case 2: return launch_wide<T, 2>(p, threads, stream);
+            case 3: return launch_wide<T, 3>(p, threads, stream);
+            case 4: return launch_wide<T, 4>(p, threads, stream);
+            case 5: return launch_wide<T, 5>(p, threads, stream);
+            default: return launch_wide<T, 6>(p, threads, stream);
+        }
+    } else if constexpr (kE == 4) {
+        if (per_thread <= 2) return launch_narrow<T, 4, 2>(p, threads, stream);
+        return launch_narrow<T, 4, 4>(p, threads, stream);
+    } else {
+        if (per_thread <= 4) return launch_narrow<T, 1, 4>(p, threads, stream);
+        if (per_thread <= 8) return launch_narrow<T, 1, 8>(p, threads, stream);
+        if (per_thread <= 12) return launch_narrow<T, 1, 12>(p, threads, stream);
+        return launch_narrow<T, 1, 16>(p, threads, stream);
     }
 }
 
