@@ -1,3 +1,3 @@
-from .layer import FP8RotateQuantFA, add_fa_quant
+from .layer import FP8DynamicLinear, FP8RotateQuantFA, add_fa_quant
 
-__all__ = ["FP8RotateQuantFA", "add_fa_quant"]
+__all__ = ["FP8DynamicLinear", "FP8RotateQuantFA", "add_fa_quant"]
