@@ -190,7 +190,7 @@ __device__ __forceinline__ void report(const LinearParams& p, const volatile int
 
 constexpr int kEpilogueWarps = 16;
 constexpr int kPairThreads = 128 + 32 * kEpilogueWarps;  // warps: 0 loader, 1 MMA, 2 tensor memory, 3 idle, 4.. epilogue
-constexpr int kSub = 2;  // k steps per ring stage: one barrier round trip and one commit for eight MMAs
+constexpr int kSub = 2;  // swap kernel: k steps per ring stage, one barrier round trip and one commit for eight MMAs
 constexpr int kRingBytes = 6 * 2 * kRowTile;  // pair kernel: three stages of 256-column tiles, more of narrower ones
 constexpr int kPairMaxStages = 8;
 // The epilogue works in units of 32 rows x 16 columns.  Four warps share a quarter of the tile's rows and take its
@@ -277,7 +277,8 @@ __device__ __forceinline__ void tile_at(const LinearParams& p, int t, int& tm, i
     tm = b * p.band + in - tn * rows;
 }
 
-template <bool kFp8>
+// kSteps: k steps per ring stage (pair_sub).
+template <bool kFp8, int kSteps>
 __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __grid_constant__ LinearParams p) {
     extern __shared__ char smem_raw[];
     char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -338,13 +339,13 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
                 tile_at(p, t, tm, tn);
                 const int row_x = tm * 256 + static_cast<int>(rank) * 128;
                 const int row_w = tn * p.tile_n + static_cast<int>(rank) * (p.tile_n / 2);
-                for (int ks = 0; ks < p.k_steps; ks += kSub) {
+                for (int ks = 0; ks < p.k_steps; ks += kSteps) {
                     ok = mbar_wait_warp(empty + 8 * stage, phase ^ 1, abort_flag, 1, limit);
                     if (!ok) break;
-                    const int subs = min(kSub, p.k_steps - ks);
+                    const int subs = min(kSteps, p.k_steps - ks);
                     if (one) {
                         if (rank == 0) mbar_arrive_expect_tx(full + 8 * stage, subs * 2 * step_bytes);
-                        uint32_t dst = ring + stage * kSub * step_bytes;
+                        uint32_t dst = ring + stage * kSteps * step_bytes;
                         for (int j = 0; j < subs; ++j, dst += step_bytes) {
                             tma_load_4d_pair(dst, &p.tm_x, full0 + 8 * stage, (ks + j) * p.k_step_elems, row_x, 0, 0);
                             tma_load_4d_pair(dst + kRowTile, &p.tm_w, full0 + 8 * stage, (ks + j) * p.k_step_elems, row_w, 0, 0);
@@ -383,15 +384,15 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t d = tmem + acc * 256;
-                for (int ks = 0; ks < p.k_steps; ks += kSub) {
+                for (int ks = 0; ks < p.k_steps; ks += kSteps) {
                     ok = mbar_wait_warp(full + 8 * stage, phase, abort_flag, 4, limit);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t a = desc_lo(ring + stage * kSub * step_bytes, 16);
-                    const uint32_t b = desc_lo(ring + stage * kSub * step_bytes + kRowTile, 16);
+                    const uint32_t a = desc_lo(ring + stage * kSteps * step_bytes, 16);
+                    const uint32_t b = desc_lo(ring + stage * kSteps * step_bytes + kRowTile, 16);
                     if (one) {
 #pragma unroll
-                        for (int j = 0; j < kSub; ++j) {
+                        for (int j = 0; j < kSteps; ++j) {
                             if (ks + j >= p.k_steps) break;
 #pragma unroll
                             for (int i = 0; i < 4; ++i)  // 32 bytes of k per MMA
@@ -399,7 +400,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
                                                    kDescHiSbo1024, p.idesc, (ks | j | i) != 0);
                         }
                         umma_commit_pair(empty + 8 * stage);
-                        if (ks + kSub >= p.k_steps) umma_commit_pair(acc_full + 8 * acc);
+                        if (ks + kSteps >= p.k_steps) umma_commit_pair(acc_full + 8 * acc);
                     }
                     __syncwarp();
                     if (++stage == p.stages) {
@@ -839,11 +840,18 @@ cudaError_t launch_clusters(const LinearParams& p, dim3 grid, int cluster, int t
     return cudaLaunchKernelEx(&launch.cfg, kKernel, p);
 }
 
+// k steps per ring stage of the pair kernel: two halve the barriers' round trips, one makes better use of the ring
+// where two of a tile's steps do not divide it (512 x 4096 x 5120 bf16: 160 columns 22.4 us with one, 24.8 with two;
+// 2048 x 5120 x 5120: 192 columns 75 and 79 us, 128 columns 94 and 86, 256 columns 89 and 85).
+constexpr int pair_sub(int tile_n) { return tile_n <= 128 || tile_n == 256 ? 2 : 1; }
+
 template <bool kFp8>
 cudaError_t launch_pair(const LinearParams& p, cudaStream_t stream) {
     const int tiles = p.tiles_m * p.tiles_n;
     const dim3 grid(2 * (tiles < kSms / 2 ? tiles : kSms / 2));
-    return launch_clusters<linear_pair_kernel<kFp8>>(p, grid, 2, kPairThreads, kPairSmem, stream);
+    return pair_sub(p.tile_n) == 1
+               ? launch_clusters<linear_pair_kernel<kFp8, 1>>(p, grid, 2, kPairThreads, kPairSmem, stream)
+               : launch_clusters<linear_pair_kernel<kFp8, 2>>(p, grid, 2, kPairThreads, kPairSmem, stream);
 }
 
 // How a product is cut up.
@@ -867,7 +875,7 @@ constexpr int swap_stages(int tile_n, int per_sm) {
     return stages < kSwapMaxStages ? stages : kSwapMaxStages;
 }
 constexpr int pair_stages(int tile_n) {
-    const int stages = kRingBytes / (kSub * (kRowTile + tile_n / 2 * kStepBytes));
+    const int stages = kRingBytes / (pair_sub(tile_n) * (kRowTile + tile_n / 2 * kStepBytes));
     return stages < kPairMaxStages ? stages : kPairMaxStages;
 }
 
@@ -937,7 +945,7 @@ Plan estimate_plan(int m, int n, int k_steps) {
     int last = 0;
     for (int want = 16; want <= kSwapMaxTile; want += 16) {
         const int64_t parts = ceil_div(m, want);
-        if (blocks_n * parts > 2 * kSms * 2) continue;
+        if (parts > 1 && blocks_n * parts > 2 * kSms * 2) continue;  // w would be read by many blocks
         const int tile = static_cast<int>(ceil_div(ceil_div(m, parts), 16) * 16);  // even parts
         if (tile == last) continue;
         last = tile;

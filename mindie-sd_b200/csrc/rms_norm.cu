@@ -663,7 +663,8 @@ using namespace sdb;
 extern "C" int mindiesd_add_rms_norm(const mindiesd_norm_args* a, void* stream_) {
     if (!a || !a->x || !a->out) return MINDIESD_E_NULL;
     if ((a->residual == nullptr) != (a->residual_out == nullptr)) return MINDIESD_E_NULL;
-    if (a->rows <= 0 || a->rows > 0x7fffffff || a->dim <= 0) return MINDIESD_E_SHAPE;
+    if (a->rows <= 0 || a->dim <= 0) return MINDIESD_E_SHAPE;
+    if (a->rows > 0x7fffffff || a->dim > 0x3fffffff) return MINDIESD_E_CAPACITY;  // blocks of a grid, 32-bit columns
     if (a->dtype != MINDIESD_BF16 && a->dtype != MINDIESD_FP16 && a->dtype != MINDIESD_FP32) return MINDIESD_E_DTYPE;
     if (a->residual && a->residual_dtype != a->dtype && a->residual_dtype != MINDIESD_FP32) return MINDIESD_E_DTYPE;
     if (a->weight && a->weight_dtype != a->dtype && a->weight_dtype != MINDIESD_FP32) return MINDIESD_E_DTYPE;

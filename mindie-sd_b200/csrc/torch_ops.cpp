@@ -840,9 +840,9 @@ std::tuple<at::Tensor, MaybeTensor, MaybeTensor> add_rms_norm_cuda(const at::Ten
     const at::ScalarType type = x.scalar_type();
     TORCH_CHECK(x.is_cuda() && x.dim() >= 1 && x.size(-1) > 0 && !records_gradients(x), "add_rms_norm: x must be a CUDA tensor [..., D]");
     TORCH_CHECK(type == at::kBFloat16 || type == at::kHalf || type == at::kFloat, "add_rms_norm: x must be bf16, fp16 or fp32");
-    TORCH_CHECK(eps > 0 && eps < 1e30, "add_rms_norm: eps must be positive");
+    TORCH_CHECK(eps > 1e-38 && eps < 1e30, "add_rms_norm: eps must be positive and normal in fp32");
     const int64_t d = x.size(-1);
-    TORCH_CHECK(d <= std::numeric_limits<int32_t>::max(), "add_rms_norm: D is too large");
+    TORCH_CHECK(d <= 0x3fffffff && x.numel() / d <= std::numeric_limits<int32_t>::max(), "add_rms_norm: too many channels or rows");
     mindiesd_norm_args a = {};
     at::Tensor xr = as_rows(x, &a.rows, &a.x_stride);
     at::Tensor rr, wr, residual_out, scales;

@@ -70,6 +70,8 @@ def _explain(x, weight, bias, activation, residual, gate, x_scale, weight_scale,
                   f"{name} must be float32 with one value in all or one per row ({count}), but got {tuple(t.shape)} in {t.dtype}.")
     else:
         _want(x_scale is None and weight_scale is None, "x_scale and weight_scale belong to e4m3 operands.")
+    _want(max(weight.shape[0], weight.shape[1], x.numel() // x.shape[-1]) <= 0x7fff0000,
+          f"Too many rows or columns: {tuple(x.shape)} and {tuple(weight.shape)}.")
     refuse_gradients("linear_forward", x, weight, bias, residual, gate, x_scale, weight_scale)
     _want(x.is_cuda or x.is_meta, f"linear_forward runs on a CUDA device, but x is on {x.device}.")
 

@@ -48,8 +48,10 @@ def _explain(where, x, weight, residual, eps):
                                     f"{tuple(residual.shape)} on {residual.device}.")
         if residual.dtype != x.dtype and residual.dtype != torch.float32:
             raise ParametersInvalid(f"The input residual must be {x.dtype} or float32, but got {residual.dtype}.")
-    if not isinstance(eps, float) or not 0.0 < eps < 1e30:
-        raise ParametersInvalid(f"The input eps must be a positive float, but got {eps!r}.")
+    if not isinstance(eps, float) or not 1e-38 < eps < 1e30:
+        raise ParametersInvalid(f"The input eps must be a positive float (normal in float32), but got {eps!r}.")
+    if x.shape[-1] > 0x3fffffff or x.numel() // x.shape[-1] > 0x7fffffff:
+        raise ParametersInvalid(f"{where} takes at most 2^30 - 1 channels and 2^31 - 1 rows, but got {tuple(x.shape)}.")
     refuse_gradients(where, x, weight, residual)
     if not x.is_cuda and not x.is_meta:
         raise ParametersInvalid(f"{where} runs on a CUDA device, but x is on {x.device}.")

@@ -16,6 +16,9 @@ def _explain(input_tensor):
     if input_tensor.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise ParametersInvalid(f"token_quant_preprocess supports bfloat16, float16 and float32, but got "
                                 f"{input_tensor.dtype}.")
+    if input_tensor.shape[-1] > 0x3fffffff or input_tensor.numel() // input_tensor.shape[-1] > 0x7fffffff:
+        raise ParametersInvalid(f"token_quant_preprocess takes at most 2^30 - 1 channels and 2^31 - 1 rows, but got "
+                                f"{tuple(input_tensor.shape)}.")
     refuse_gradients("token_quant_preprocess", input_tensor)
     if not input_tensor.is_cuda and not input_tensor.is_meta:
         raise ParametersInvalid(f"token_quant_preprocess runs on a CUDA device, but input_tensor is on "

@@ -82,26 +82,43 @@ def test_struct_layout_and_codes_without_a_gpu(tmp_path):
             ctypes.sizeof(_cabi.NormArgs)
 
 
-def test_refusals():
+def _refused(device):
+    x = torch.zeros(4, 64, dtype=torch.bfloat16, device=device)
+    return x, [
+        dict(x=[1.0]), dict(x=x.double()), dict(x=torch.zeros(4, 0, dtype=torch.bfloat16, device=device)),
+        dict(x=torch.zeros((), device=device)), dict(x=torch.zeros(4, 64)),  # not on a CUDA device
+        dict(x=x, weight=torch.zeros(63, device=device)), dict(x=x, weight=torch.zeros(64, dtype=torch.float16, device=device)),
+        dict(x=x, weight=torch.zeros(64)), dict(x=x, weight=3.0), dict(x=x, weight=torch.zeros(1, 64, device=device)),
+        dict(x=x, residual=x[:3]), dict(x=x, residual=x.half()), dict(x=x, residual=torch.zeros(4, 64)), dict(x=x, residual=0),
+        dict(x=x, eps=0.0), dict(x=x, eps=-1e-6), dict(x=x, eps=1e-50), dict(x=x, eps=float("nan")), dict(x=x, eps="1"),
+        dict(x=x, weight=torch.zeros(64, device=device, requires_grad=True)), dict(x=x.clone().requires_grad_()),
+        dict(x=x, residual=x.clone().requires_grad_()),
+    ]
+
+
+def _check_refusals(device):
     from mindiesd import ParametersInvalid, add_rms_norm, add_rms_norm_quant
     from mindiesd.layers.quant import token_quant_preprocess
-    x = torch.zeros(4, 64, dtype=torch.bfloat16, device="meta")
-    bad = [
-        dict(x=[1.0]), dict(x=x.double()), dict(x=torch.zeros(4, 0, dtype=torch.bfloat16, device="meta")),
-        dict(x=torch.zeros(4, 64)),  # not on a CUDA device
-        dict(x=x, weight=torch.zeros(63, device="meta")), dict(x=x, weight=torch.zeros(64, dtype=torch.float16, device="meta")),
-        dict(x=x, weight=torch.zeros(64)), dict(x=x, weight=3.0),
-        dict(x=x, residual=x[:3]), dict(x=x, residual=x.half()), dict(x=x, residual=torch.zeros(4, 64)), dict(x=x, residual=0),
-        dict(x=x, eps=0.0), dict(x=x, eps=-1e-6), dict(x=x, eps=1), dict(x=x, eps=float("nan")),
-        dict(x=x, weight=torch.zeros(64, device="meta", requires_grad=True)),
-    ]
-    for kw in bad:
+    x, bad = _refused(device)
+    for i, kw in enumerate(bad):
         for fn in (add_rms_norm, add_rms_norm_quant):
             with pytest.raises(ParametersInvalid):
                 fn(**kw)
-    for t in ([1.0], torch.zeros(4, 64), x.double(), torch.zeros((), device="meta"), x.float().requires_grad_()):
+                pytest.fail(f"call {i} was taken")
+    for t in ([1.0], torch.zeros(4, 64), x.double(), torch.zeros((), device=device), x.float().requires_grad_()):
         with pytest.raises(ParametersInvalid):
             token_quant_preprocess(t)
+    with torch.no_grad():
+        assert add_rms_norm(x, torch.nn.Parameter(torch.zeros(64, device=device))).shape == x.shape
+
+
+def test_refusals():
+    _check_refusals("meta")
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_device():
+    _check_refusals("cuda")
 
 
 def test_fake_shapes():

@@ -80,11 +80,10 @@ def test_codes_without_a_gpu(tmp_path):
             ctypes.sizeof(_cabi.LinearArgs)
 
 
-def test_refusals():
-    from mindiesd import ParametersInvalid, linear_forward
-
+def _refused(device):
+    """(calls that are refused, calls that are not) with every tensor on `device`."""
     def t(*shape, dtype=torch.bfloat16):
-        return torch.zeros(shape, dtype=dtype, device="meta")
+        return torch.zeros(shape, dtype=dtype, device=device)
     x, w = t(2, 5, 64), t(32, 64)
     x8, w8 = t(2, 5, 64, dtype=torch.float8_e4m3fn), t(32, 64, dtype=torch.float8_e4m3fn)
     s, ws = t(2, 5, 1, dtype=torch.float32), t(32, dtype=torch.float32)
@@ -97,29 +96,57 @@ def test_refusals():
         dict(x=x, weight=w, bias=t(33)), dict(x=x, weight=w, bias=t(1, 32)), dict(x=x, weight=w, bias=t(32, dtype=torch.float64)),
         dict(x=x, weight=w, bias=torch.zeros(32)), dict(x=x, weight=w, bias=0.0),
         dict(x=x, weight=w, residual=t(2, 5, 33)), dict(x=x, weight=w, residual=t(10, 32)), dict(x=x, weight=w, residual=t(2, 5, 32).half()),
+        dict(x=x, weight=w, residual=torch.zeros(2, 5, 32, dtype=torch.bfloat16)),
         dict(x=x, weight=w, gate=t(31)), dict(x=x, weight=w, gate=t(3, 1, 32)), dict(x=x, weight=w, gate=t(2, 5, 32)),
         dict(x=x, weight=w, gate=t(5, 32)), dict(x=x, weight=w, gate=t(32, dtype=torch.int32)), dict(x=t(64), weight=w, gate=t(2, 32)),
         dict(x=x, weight=w, x_scale=s, weight_scale=ws), dict(x=x8, weight=w8), dict(x=x8, weight=w8, x_scale=s),
         dict(x=x8, weight=w, x_scale=s, weight_scale=ws), dict(x=x8, weight=w8, x_scale=s.half(), weight_scale=ws),
         dict(x=x8, weight=w8, x_scale=t(10, dtype=torch.float32), weight_scale=ws),
         dict(x=x8, weight=w8, x_scale=s, weight_scale=t(31, dtype=torch.float32)),
-        dict(x=x8, weight=w8, x_scale=s, weight_scale=1.0),
-        dict(x=x, weight=torch.nn.Parameter(w)),
+        dict(x=x8, weight=w8, x_scale=s, weight_scale=1.0), dict(x=x8, weight=w8, x_scale=s, weight_scale=torch.zeros(32)),
+        dict(x=x8, weight=w8, x_scale=s, weight_scale=ws, residual=t(2, 5, 32, dtype=torch.float32)),
+        dict(x=x, weight=torch.nn.Parameter(w)), dict(x=x, weight=w, bias=t(32).requires_grad_()),
+        dict(x=x.clone().requires_grad_(), weight=w), dict(x=x, weight=w, gate=t(32).requires_grad_()),
     ]
+    good = [dict(x=x, weight=w), dict(x=x8, weight=w8, x_scale=s, weight_scale=ws), dict(x=x, weight=w, gate=t(1, 1, 1, 32)),
+            dict(x=x8, weight=w8, x_scale=s[..., 0], weight_scale=ws[:, None], residual=t(2, 5, 32).half())]
+    return bad, good
+
+
+def test_refusals():
+    from mindiesd import ParametersInvalid, linear_forward
+    bad, good = _refused("meta")
     for kw in bad:
         with pytest.raises(ParametersInvalid):
             linear_forward(**kw)
-    assert linear_forward(x, w).shape == (2, 5, 32) and linear_forward(x8, w8, x_scale=s, weight_scale=ws).dtype == torch.bfloat16
-    assert linear_forward(x8, w8, x_scale=s[..., 0], weight_scale=ws[:, None], residual=t(2, 5, 32).half()).dtype == torch.float16
+    assert [linear_forward(**kw).dtype for kw in good] == [torch.bfloat16, torch.bfloat16, torch.bfloat16, torch.float16]
+    assert all(linear_forward(**kw).shape == (2, 5, 32) for kw in good)
     with torch.no_grad():
-        assert linear_forward(t(64), torch.nn.Parameter(w)).shape == (32,)
+        assert linear_forward(good[0]["x"][0, 0], torch.nn.Parameter(good[0]["weight"])).shape == (32,)
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_device():
+    """The operator makes the checks itself on the way to the kernel; nothing is launched for a refused call."""
+    from mindiesd import ParametersInvalid, linear_forward
+    bad, good = _refused("cuda")
+    for i, kw in enumerate(bad):
+        with pytest.raises(ParametersInvalid):
+            linear_forward(**kw)
+            pytest.fail(f"call {i} was taken")
+    for kw in good:
+        assert linear_forward(**kw).shape == (2, 5, 32)
+    torch.cuda.synchronize()
 
 
 # ---- GPU -------------------------------------------------------------------------------------------
 
+# Both kernels, one and several blocks or tiles along every side, shares of k down to a step, every width of tile.
 SHAPES = [(1, 256, 5120), (2, 64, 16), (1, 1, 1), (3, 8, 130), (16, 1001, 129), (17, 200, 1000), (64, 1536, 1536), (100, 4096, 257),
           (128, 72, 256), (129, 72, 256), (200, 520, 33), (256, 64, 256), (257, 1024, 1000), (300, 1536, 1001), (513, 5120, 640),
-          (1000, 333, 514), (2048, 128, 2048), (5000, 256, 96)]
+          (1000, 333, 514), (2048, 128, 2048), (5000, 256, 96),
+          (1, 20480, 640), (33, 9000, 700), (150, 2000, 1100), (260, 15000, 100), (512, 1024, 2560), (1100, 512, 3500),
+          (1500, 64, 9000), (4100, 768, 24), (700, 1536, 6144), (2500, 640, 5000)]
 
 
 @pytest.mark.gpu
@@ -271,3 +298,46 @@ def test_offsets_beyond_32_bits():
     out = linear_forward(x, w)  # 2.25e9 elements
     _check(out[-2:], x[-2:], w, torch.bfloat16, 64)
     assert torch.count_nonzero(out[-300:-2]).item() == 0
+
+
+@pytest.mark.gpu
+def test_first_calls_of_a_process_may_be_captured():
+    """Nothing that the operators set up once (limits, tables) needs a call before the capture."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    root = Path(__file__).resolve().parent.parent
+    code = (
+        "import sys, torch; sys.path.insert(0, 'mindie-sd_b200')\n"
+        "from mindiesd import add_rms_norm_quant, linear_forward\n"
+        "x, w = torch.ones(700, 512, device='cuda', dtype=torch.bfloat16), torch.ones(256, 512, device='cuda', dtype=torch.bfloat16)\n"
+        "torch.cuda.synchronize(); g = torch.cuda.CUDAGraph()\n"
+        "with torch.cuda.graph(g):\n"
+        "    a, b, (q, s) = linear_forward(x, w), linear_forward(x[:3], w), add_rms_norm_quant(x)\n"
+        "g.replay(); torch.cuda.synchronize()\n"
+        "assert (a == 512).all() and (b == 512).all() and (q.float() * s - 1).abs().max() < 1e-5\n"
+        "print('captured')\n")
+    run = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=200)
+    assert run.returncode == 0 and "captured" in run.stdout, run.stderr[-2000:]
+
+
+@pytest.mark.gpu
+def test_threads_call_at_once():
+    """Calls of different sizes from several host threads, each on its own stream."""
+    import threading
+    from mindiesd import linear_forward
+    work = [_operands(80 + i, m, 512, n, torch.bfloat16)[:2] for i, (m, n) in enumerate([(1, 640), (300, 256), (40, 1000), (900, 128)])]
+    want = [linear_forward(x, w) for x, w in work]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def loop(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(30):
+                if not torch.equal(linear_forward(*work[i]), want[i]):
+                    wrong.append(i)
+    threads = [threading.Thread(target=loop, args=(i,)) for i in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not wrong
