@@ -309,12 +309,14 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
         abort_flag[0] = abort_flag[1] = 0;
         tma_prefetch_desc(&p.tm_x);
         tma_prefetch_desc(&p.tm_w);
-        *dead = p.status && *reinterpret_cast<volatile int*>(p.status) != 0;
     }
+    allow_next_kernel();
     if (warp == 2) {
         tmem_alloc_pair(smem_u32(tmem_slot), 512);
         tmem_relinquish_pair();
     }
+    wait_for_kernels_before();
+    if (threadIdx.x == 0) *dead = p.status && *reinterpret_cast<volatile int*>(p.status) != 0;
     tc_fence_before();
     __syncthreads();
     cluster_sync_all();
@@ -609,10 +611,12 @@ __global__ void __launch_bounds__(kSwapThreads) linear_swap_kernel(const __grid_
         tma_prefetch_desc(&p.tm_x);
         tma_prefetch_desc(&p.tm_w);
     }
+    allow_next_kernel();
     if (warp == 1) {
         tmem_alloc(smem_u32(tmem_slot), p.tmem_cols);
         tmem_relinquish();
     }
+    wait_for_kernels_before();
     tc_fence_before();
     const bool dead = __syncthreads_or(threadIdx.x == 0 && p.status && *reinterpret_cast<volatile int*>(p.status) != 0);
     tc_fence_after();
@@ -800,21 +804,23 @@ __global__ void __launch_bounds__(kSwapThreads) linear_swap_kernel(const __grid_
 constexpr int kSms = 148;
 constexpr int kMaxSmem = 227 * 1024;
 
-// A launch configuration whose clusters span the x dimension.
+// A launch configuration whose clusters span the x dimension, and whose start may overlap the kernel before it.
 struct ClusterLaunch {
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     cudaLaunchConfig_t cfg = {};
     ClusterLaunch(dim3 grid, int cluster, int threads, int smem, cudaStream_t stream) {
         attr[0].id = cudaLaunchAttributeClusterDimension;
         attr[0].val.clusterDim.x = cluster;
         attr[0].val.clusterDim.y = 1;
         attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
         cfg.gridDim = grid;
         cfg.blockDim = dim3(threads, 1, 1);
         cfg.dynamicSmemBytes = smem;
         cfg.stream = stream;
         cfg.attrs = attr;
-        cfg.numAttrs = 1;
+        cfg.numAttrs = 2;
     }
 };
 

@@ -116,6 +116,16 @@ __device__ __forceinline__ bool mbar_wait_drain(uint32_t bar, uint32_t parity, u
 }
 
 // ----------------------------------------------------------------------------------------------
+// Overlap of a kernel's start with the end of the one before it in the stream (launches that carry
+// cudaLaunchAttributeProgrammaticStreamSerialization; without the attribute both do nothing)
+// ----------------------------------------------------------------------------------------------
+// The next kernel may be brought onto the SMs from now on.
+__device__ __forceinline__ void allow_next_kernel() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// Returns once the kernels before this one are complete and what they wrote is visible.  Every thread passes it before
+// its first access to global memory, reads and writes alike.
+__device__ __forceinline__ void wait_for_kernels_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// ----------------------------------------------------------------------------------------------
 // TMA (tiled bulk tensor loads, each CTA fetching its own tiles)
 // ----------------------------------------------------------------------------------------------
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* m) {

@@ -118,6 +118,8 @@ __device__ __forceinline__ void weights_of(const NormParams& p, int at, float (&
 // Few rows that start on 16-byte boundaries: one row per `group` threads, kV runs of 16 bytes per thread.
 template <typename T, int kE, int kV>
 __global__ void __launch_bounds__(1024) norm_row_kernel(const NormParams p) {
+    allow_next_kernel();
+    wait_for_kernels_before();
     const int lane = threadIdx.x & (p.group - 1);
     const int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x / p.group) + threadIdx.x / p.group;
     const bool live = row < p.rows;  // the threads of a missing row still take part in the shuffles
@@ -313,6 +315,8 @@ __global__ void __launch_bounds__(kRes > 0 ? 512 : 768) norm_stream_kernel(const
     for (int slot = 0; slot < kAhead; ++slot)
         for (int j = runs; j < kV; ++j)
             for (int q = 0; q < kPieces; ++q) store_shared16(place(slot, j, q), make_uint4(0, 0, 0, 0));
+    allow_next_kernel();
+    wait_for_kernels_before();
     for (int i = 0; i < kAhead; ++i) fetch(first + i * step, i);
     int slot = 0, turn = 0;
     // Every thread of the block makes the same number of rounds: the reduction of wide groups is a block barrier.
@@ -435,6 +439,8 @@ __global__ void __launch_bounds__(512) norm_narrow_kernel(const NormParams p) {
             if constexpr (kRes > 0) add[j].load(r + at);
         }
     };
+    allow_next_kernel();
+    wait_for_kernels_before();
     fetch(first);
     float w[kV][kE];  // a load of them within the loop would have to wait for the next row's runs as well
 #pragma unroll
@@ -489,6 +495,8 @@ __global__ void __launch_bounds__(512) norm_narrow_kernel(const NormParams p) {
 // Rows too long for the registers of a block: one block per row, the row read twice (the second time from L2).
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_long_kernel(const NormParams p) {
+    allow_next_kernel();
+    wait_for_kernels_before();
     const int64_t row = blockIdx.x;
     const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
     auto value = [&](int at) {
@@ -529,6 +537,21 @@ constexpr int kStreamBlocks = 4 * kSms;
 
 constexpr int kMaxSmem = 226 * 1024;  // of 227 KB, beside the partials of the reduction
 
+// A launch whose start may overlap the end of the kernel before it (each kernel waits before its first access to memory).
+cudaError_t launch(void (*kernel)(NormParams), const NormParams& p, int64_t blocks, int threads, int smem, cudaStream_t stream) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
 template <int kV, int kRes>
 constexpr int stream_smem(int threads) { return kAhead * kV * (16 + kRes) * threads; }
 
@@ -552,8 +575,7 @@ cudaError_t launch_stream_as(const NormParams& p, int threads, cudaStream_t stre
         known.store(per_sm, std::memory_order_release);
     }
     const int64_t blocks = (p.rows + threads / p.group - 1) / (threads / p.group);
-    kernel<<<static_cast<unsigned>(std::min<int64_t>(blocks, static_cast<int64_t>(kSms) * per_sm)), threads, smem, stream>>>(p);
-    return cudaGetLastError();
+    return launch(kernel, p, std::min<int64_t>(blocks, static_cast<int64_t>(kSms) * per_sm), threads, smem, stream);
 }
 
 template <typename T, int kE, int kV, int kRes>
@@ -578,18 +600,16 @@ cudaError_t launch_wide(const NormParams& p, int threads, cudaStream_t stream) {
             if (stream_smem<kV, 16>(threads) <= kMaxSmem) return launch_stream<T, kE, kV, 16>(p, threads, stream);
         }
     }
-    norm_row_kernel<T, kE, kV><<<static_cast<unsigned>(blocks), threads, 0, stream>>>(p);
-    return cudaGetLastError();
+    return launch(norm_row_kernel<T, kE, kV>, p, blocks, threads, 0, stream);
 }
 
 template <typename T, int kE, int kV>
 cudaError_t launch_narrow(const NormParams& p, int threads, cudaStream_t stream) {
     const int64_t blocks = (p.rows + threads / p.group - 1) / (threads / p.group);
-    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(blocks, kSms * (1024 / threads)));
-    if (!p.residual) norm_narrow_kernel<T, kE, kV, 0><<<grid, threads, 0, stream>>>(p);
-    else if (!p.residual_fp32) norm_narrow_kernel<T, kE, kV, 1><<<grid, threads, 0, stream>>>(p);
-    else norm_narrow_kernel<T, kE, kV, 2><<<grid, threads, 0, stream>>>(p);
-    return cudaGetLastError();
+    const int64_t grid = std::min<int64_t>(blocks, kSms * (1024 / threads));
+    if (!p.residual) return launch(norm_narrow_kernel<T, kE, kV, 0>, p, grid, threads, 0, stream);
+    if (!p.residual_fp32) return launch(norm_narrow_kernel<T, kE, kV, 1>, p, grid, threads, 0, stream);
+    return launch(norm_narrow_kernel<T, kE, kV, 2>, p, grid, threads, 0, stream);
 }
 
 template <typename T, int kE>
@@ -609,8 +629,7 @@ cudaError_t launch_rows(NormParams p, cudaStream_t stream) {
     }
     if (per_thread > (kWide ? 6 : most)) {
         p.group = 1024;
-        norm_long_kernel<T><<<static_cast<unsigned>(p.rows), 1024, 0, stream>>>(p);
-        return cudaGetLastError();
+        return launch(norm_long_kernel<T>, p, p.rows, 1024, 0, stream);
     }
     p.group = group;
     const int threads = group > 128 ? group : 128;

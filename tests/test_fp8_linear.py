@@ -139,3 +139,42 @@ def test_block(b, s, quantised):
     x.copy_(tn._randn(14, b, s, dim, dtype=t))
     graph.replay()
     assert torch.equal(captured, _block(x, shift, p, heads, quantised)["x2"])
+
+
+@pytest.mark.gpu
+def test_calls_back_to_back():
+    """The start of each kernel may overlap the end of the one before it.  A chain in which every call reads what
+    the call before has just written, into memory that an earlier one has just read, gives the same bits as
+    the chain with a synchronisation after every call -- eager, and replayed as one graph."""
+    from mindiesd import add_rms_norm, linear_forward
+    from mindiesd.layers.quant import token_quant_preprocess
+    for m in (1, 70, 600):
+        w1, w2 = tn._randn(1, 1024, 256, dtype=torch.bfloat16, scale=1 / 16), tn._randn(2, 256, 1024, dtype=torch.bfloat16, scale=1 / 32)
+        w8, ws = token_quant_preprocess(w2)
+        start = tn._randn(3, m, 256, dtype=torch.bfloat16)
+
+        def chain(x, pause):
+            total = x
+            for _ in range(12):
+                y, total = add_rms_norm(x, None, total)
+                pause()
+                h = linear_forward(y, w1, activation="silu")
+                pause()
+                q, s = token_quant_preprocess(h)
+                pause()
+                x = linear_forward(q, w8, x_scale=s, weight_scale=ws, residual=total)
+                pause()
+                x = x + 0.5 * linear_forward(h, w2)  # torch's own kernels in between
+                pause()
+                del y, h, q, s
+            return x
+        want = chain(start, torch.cuda.synchronize)
+        for _ in range(5):
+            assert torch.equal(chain(start, lambda: None), want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = chain(start, lambda: None)
+        for _ in range(5):
+            got.zero_()
+            graph.replay()
+            assert torch.equal(got, want)
