@@ -885,6 +885,17 @@ constexpr int pair_stages(int tile_n) {
     return stages < kPairMaxStages ? stages : kPairMaxStages;
 }
 
+// Row tiles of a band (tile_at).  All of w passes by once per band, so where w does not stay in L2 the band is as high
+// as its rows of x leave room for (32760 x 5120 x 20480 bf16 under the power cap, w 210 MB: 4 tiles 5.66 ms, 8 tiles
+// 5.29, 16 tiles 5.18); where it does, a low band keeps the tiles in flight close (32768 x 5120 x 5120 e4m3, w 26 MB:
+// 4 tiles 694 us, 16 tiles 709).
+constexpr int pair_band(int n, int k_steps) {
+    const int64_t row_bytes = static_cast<int64_t>(k_steps) * kStepBytes;
+    if (n * row_bytes <= (40 << 20)) return 4;
+    const int64_t band = (44 << 20) / (256 * row_bytes);
+    return band < 4 ? 4 : band > 16 ? 16 : static_cast<int>(band);
+}
+
 // Clusters of 1..8 blocks that the device holds at once with one and with two blocks per SM.  A cluster lies inside
 // one group of SMs, so these are not 148 / size: measured 15 of eight blocks, not 18, and a 16th one is a second wave.
 struct Residency {
@@ -944,7 +955,7 @@ Plan estimate_plan(int m, int n, int k_steps) {
         const double us = 3.28 + overlap(waves * std::max(k_steps * step, units), bytes / kMemory, 0.127) + 0.236 * units + 1.16 * waves;
         if (us < best_us) {
             best_us = us;
-            best = {false, tile_n, pair_stages(tile_n), 1, 8};
+            best = {false, tile_n, pair_stages(tile_n), 1, pair_band(n, k_steps)};
         }
     }
     const int64_t blocks_n = ceil_div(n, 128);
