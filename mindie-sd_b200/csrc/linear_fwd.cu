@@ -931,11 +931,12 @@ const Residency& residency() {
 
 // The plan with the smallest estimated time.  The estimates are a model of the two kernels (microseconds) whose
 // constants were fitted to 12 900 timings of 300 products (m 1..16000, k 64..20480, n 16..20480, both operand
-// widths, operands in HBM): the plan it picks is 1.2 % slower than the best measured one on average, and more
-// than 10 % slower for 17 of the 300.  What it weighs, with both sides measured (bf16, k 5120, n 5120):
+// widths): the plan it picks is 1.8 % slower than the best measured one on average, on 300 other products too, and
+// more than 10 % slower for one in twenty.  What it weighs, with both sides measured (bf16, k 5120, n 5120):
 //   m 64:   swap, 3 blocks per tile 16.0 us, 8 blocks 23 us (clusters of a second wave); pair 21.3 us
 //   m 256:  pair, 96 columns (54 tiles) 21.3 us, 256 columns (20 tiles) 32 us; swap 26.3 us
-//   m 2048: pair, 192 columns (216 tiles, 2.92 waves) 78 us, 256 columns (160 tiles, 2.16 waves) 94 us
+//   m 2048: pair, 192 columns (216 tiles, 2.92 waves) 75 us, 256 columns (160 tiles, 2.16 waves) 85 us
+// (Two launches, the columns of the full waves and then the rest, gained at most 8 % and lost as often.)
 Plan estimate_plan(int m, int n, int k_steps) {
     auto ceil_div = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
     const double bytes = (static_cast<double>(m) + n) * k_steps * kStepBytes + 2.0 * m * n;
@@ -962,7 +963,7 @@ Plan estimate_plan(int m, int n, int k_steps) {
     int last = 0;
     for (int want = 16; want <= kSwapMaxTile; want += 16) {
         const int64_t parts = ceil_div(m, want);
-        if (parts > 1 && blocks_n * parts > 2 * kSms * 2) continue;  // w would be read by many blocks
+        if (blocks_n > 65535 || (parts > 1 && blocks_n * parts > 2 * kSms * 2)) continue;  // (the grid; w read by many blocks)
         const int tile = static_cast<int>(ceil_div(ceil_div(m, parts), 16) * 16);  // even parts
         if (tile == last) continue;
         last = tile;
