@@ -930,7 +930,7 @@ const Residency& residency() {
 }
 
 // The plan with the smallest estimated time.  The estimates are a model of the two kernels (microseconds) whose
-// constants were fitted to 12 900 timings of 300 products (m 1..16000, k 64..20480, n 16..20480, both operand
+// constants were fitted to 8700 timings of 300 products (m 1..16000, k 64..20480, n 16..20480, both operand
 // widths): the plan it picks is 1.8 % slower than the best measured one on average, on 300 other products too, and
 // more than 10 % slower for one in twenty.  What it weighs, with both sides measured (bf16, k 5120, n 5120):
 //   m 64:   swap, 3 blocks per tile 16.0 us, 8 blocks 23 us (clusters of a second wave); pair 21.3 us
@@ -1015,7 +1015,7 @@ cudaError_t launch_swap(const LinearParams& p, cudaStream_t stream) {
 
 using namespace sdb;
 
-extern "C" int mindiesd_linear_fwd(const mindiesd_linear_args* a, void* stream_) {
+extern "C" int mindiesd_linear_fwd(const mindiesd_linear_args* a, void* stream_) try {
     if (!a || !a->x || !a->weight || !a->out) return MINDIESD_E_NULL;
     if (a->m <= 0 || a->n <= 0 || a->k <= 0) return MINDIESD_E_SHAPE;
     if (a->m > 0x7fff0000 || a->n > 0x7fff0000 || a->k > 0x7fff0000) return MINDIESD_E_CAPACITY;  // tile coordinates are 32-bit
@@ -1097,5 +1097,9 @@ extern "C" int mindiesd_linear_fwd(const mindiesd_linear_args* a, void* stream_)
         if ((rc = encode_tile_map(&p.tm_w, a->weight, a->in_dtype, a->k, a->n, 1, 1, w_strides, p.tile_n / 2))) return rc;
         err = fp8 ? launch_pair<true>(p, stream) : launch_pair<false>(p, stream);
     }
-    return err == cudaSuccess ? MINDIESD_OK : static_cast<int>(err);
+    if (err == cudaSuccess) return MINDIESD_OK;
+    cudaGetLastError();  // the caller gets the error from here; the next call's check must not find it again
+    return static_cast<int>(err);
+} catch (...) {  // a lock that the system refused; nothing may cross this boundary
+    return MINDIESD_E_DRIVER;
 }

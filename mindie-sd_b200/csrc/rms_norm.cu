@@ -743,5 +743,7 @@ extern "C" int mindiesd_add_rms_norm(const mindiesd_norm_args* a, void* stream_)
     if (a->dtype == MINDIESD_BF16) err = launch_typed<__nv_bfloat16>(p, stream);
     else if (a->dtype == MINDIESD_FP16) err = launch_typed<__half>(p, stream);
     else err = launch_typed<float>(p, stream);
-    return err == cudaSuccess ? MINDIESD_OK : static_cast<int>(err);
+    if (err == cudaSuccess) return MINDIESD_OK;
+    cudaGetLastError();  // the caller gets the error from here; the next call's check must not find it again
+    return static_cast<int>(err);
 }

@@ -73,7 +73,7 @@ def add_rms_norm(x, weight=None, residual=None, eps=1e-6):
     without a residual) and one rounding to the type of x.  x: [..., D] bf16, fp16 or fp32; weight [D] (None:
     ones) and residual [..., D] in the type of x or fp32.  Returns y, or (y, v rounded to the residual's type)
     when a residual is given.  Leading dimensions that share one row stride (slices of a packed projection)
-    are read in place."""
+    are read in place.  The squares are summed in fp32: values beyond 1.8e19 overflow it and give a row of zeros."""
     y, _, total = _run("add_rms_norm", x, weight, residual, eps, False)
     return y if residual is None else (y, total)
 

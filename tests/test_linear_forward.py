@@ -341,3 +341,74 @@ def test_threads_call_at_once():
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert not wrong
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n", [(1, 136), (7, 136), (100, 131), (300, 200), (300, 131), (515, 520)])
+def test_strided_output_leaves_the_rest_alone(m, n):
+    """Through the C ABI: an output whose rows lie in wider ones, residual and gate with strides of their own; columns and
+    rows beyond the product keep what they held."""
+    from mindiesd import _cabi
+    k = 192
+    x, w, _ = _operands(90, m, k, n, torch.bfloat16)
+    for start, pad in ((0, 24), (8, 40), (3, 17)):
+        wide = torch.full((m + 5, n + pad), 7.0, dtype=torch.bfloat16, device="cuda")
+        out = wide[2:2 + m, start:start + n]
+        r, g = _randn(91, m, n + 9, dtype=torch.bfloat16)[:, 1:1 + n], _randn(92, m, n + 3)[:, :n]
+        a = _cabi.LinearArgs()
+        a.x, a.weight, a.out, a.residual, a.gate = x.data_ptr(), w.data_ptr(), out.data_ptr(), r.data_ptr(), g.data_ptr()
+        a.x_stride = a.weight_stride = k
+        a.out_stride, a.residual_stride, a.gate_stride = wide.stride(0), r.stride(0), g.stride(0)
+        a.m, a.n, a.k, a.rows_per_gate = m, n, k, 1
+        a.in_dtype = a.out_dtype = _cabi.BF16
+        a.gate_dtype = _cabi.FP32
+        _cabi.check(_cabi.lib().mindiesd_linear_fwd(ctypes.byref(a), _cabi.current_stream_ptr(x.device)), "mindiesd_linear_fwd")
+        _check(out, x, w, torch.bfloat16, k, residual=r, gate=g)
+        keep = torch.ones_like(wide, dtype=torch.bool)
+        keep[2:2 + m, start:start + n] = False
+        assert (wide[keep] == 7).all()
+
+
+@pytest.mark.gpu
+def test_fork_and_join_in_a_graph():
+    """Calls with several predecessors: a captured side stream that joins the main one."""
+    from mindiesd import add_rms_norm, linear_forward
+    for m in (3, 400):
+        x, w, _ = _operands(95, m, 256, 256, torch.bfloat16)
+
+        def run():
+            main = torch.cuda.current_stream()
+            y = add_rms_norm(x)
+            side.wait_stream(main)
+            with torch.cuda.stream(side):
+                z = linear_forward(y, w)
+            u = linear_forward(y, w, activation="silu")
+            main.wait_stream(side)
+            return add_rms_norm(linear_forward(u, w, residual=z), None, z)[1]
+        side = torch.cuda.Stream()
+        want = run()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = run()
+        for _ in range(3):
+            got.zero_()
+            graph.replay()
+            assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_failed_launch_leaves_no_error_behind():
+    """An address that the copy engine cannot take is refused by its code, and the next call is not disturbed."""
+    from mindiesd import _cabi, linear_forward
+    x, w, _ = _operands(97, 8, 64, 64, torch.bfloat16)
+    out = torch.zeros(8, 64, dtype=torch.bfloat16, device="cuda")
+    a = _cabi.LinearArgs()
+    a.x, a.weight, a.out = x.data_ptr() + 2, w.data_ptr(), out.data_ptr()
+    a.x_stride = a.weight_stride = a.out_stride = 64
+    a.m, a.n, a.k = 7, 64, 64
+    a.in_dtype = a.out_dtype = _cabi.BF16
+    assert _cabi.lib().mindiesd_linear_fwd(ctypes.byref(a), _cabi.current_stream_ptr(x.device)) == -4
+    torch.cuda.synchronize()
+    assert torch.count_nonzero(out).item() == 0
+    _check(linear_forward(x, w), x, w, torch.bfloat16, 64)
