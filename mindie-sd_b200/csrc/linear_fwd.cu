@@ -6,7 +6,7 @@
 //
 // `linear_pair_kernel` (many rows): persistent, two thread blocks (a cluster on neighbouring SMs) work on one
 // 256 x tile_n tile with two-SM MMAs, so each SM fetches 128 rows of x and only HALF of the tile's rows of w: 32 KB
-// per 128 x 256 x 128-byte step.  Two accumulators of up to 256 columns: the epilogue of a tile (eight warps per block)
+// per 128 x 256 x 128-byte step.  Two accumulators of up to 256 columns: the epilogue of a tile (16 warps per block)
 // runs under the MMAs of the next one.
 //
 // `linear_swap_kernel` (few rows): the time is that of reading w once, so w takes the M side of the MMA (128 of

@@ -82,6 +82,20 @@ def test_struct_layout_and_codes_without_a_gpu(tmp_path):
             ctypes.sizeof(_cabi.NormArgs)
 
 
+@pytest.mark.parametrize("written,read", [("out", "x"), ("out", "residual"), ("residual_out", "x"), ("residual_out", "residual")])
+def test_outputs_over_inputs_are_refused(written, read):
+    """Addresses that overlap by one element; refused before anything reads them, so no device is needed."""
+    from mindiesd import _cabi
+    for delta in (0, 2 * (3 * 80 + 64) - 2, -(2 * 4 * 64 - 2)):  # the same address, the input's last element, its first
+        a = _cabi.NormArgs()
+        a.rows, a.dim, a.eps = 4, 64, 1e-6
+        a.dtype = a.out_dtype = a.residual_dtype = _cabi.BF16
+        a.x, a.residual, a.out, a.residual_out = 1 << 20, 2 << 20, 3 << 20, 4 << 20
+        a.x_stride = a.residual_stride = 80
+        setattr(a, written, getattr(a, read) + delta)
+        assert _cabi.lib().mindiesd_add_rms_norm(ctypes.byref(a), None) == -5
+
+
 def _refused(device):
     x = torch.zeros(4, 64, dtype=torch.bfloat16, device=device)
     return x, [
