@@ -529,6 +529,23 @@ typedef struct mindiesd_linear_args {
 int mindiesd_linear_fwd(const mindiesd_linear_args* args, void* stream);
 
 /*
+ * Copies `rows` rows of row_bytes bytes, src_stride bytes apart (0: one row, repeated), to rows dst_stride bytes
+ * apart: lays operands out for mindiesd_linear_fwd that do not start on 16 bytes, or that start on 16 but not on
+ * 32 bytes (it takes those, but fetches them at a lower rate).  dst and dst_stride are multiples of 16; the bytes from
+ * a row's end to the next multiple of 16 are set to zero, those behind it are left.  src and dst must not overlap.
+ */
+typedef struct mindiesd_copy_rows_args {
+    const void* src;
+    void* dst;
+    int64_t rows;
+    int64_t row_bytes;
+    int64_t src_stride;
+    int64_t dst_stride;
+} mindiesd_copy_rows_args;
+
+int mindiesd_copy_rows(const mindiesd_copy_rows_args* args, void* stream);
+
+/*
  * The re-shard step of Ulysses sequence parallelism as one data-movement kernel.
  *
  * A rank holds `rows` tokens with all N heads: tensors [rows, N, 128] addressed by a row and a head

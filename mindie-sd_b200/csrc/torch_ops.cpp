@@ -889,17 +889,60 @@ std::tuple<at::Tensor, MaybeTensor, MaybeTensor> add_rms_norm_cuda(const at::Ten
 }
 
 // ---- matrix product with bias, activation, gate and residual ------------------------------------------------
-// Rows as the copy engine fetches them: 16-byte aligned, a multiple of 16 bytes apart, not overlapping.  Anything else
-// (an uneven width, a broadcast, an odd slice) is copied once to rows of a padded stride.
-at::Tensor as_tma_rows(const at::Tensor& x, int64_t* rows, int64_t* stride) {
-    at::Tensor r = as_rows(x, rows, stride);
+// An operand as the copy engine fetches it: rows that are 16-byte aligned, a multiple of 16 bytes apart, not overlapping.
+struct TmaRows {
+    at::Tensor t;
+    int64_t rows = 0, stride = 0;
+    bool fits = false;  // as it is
+    bool slow = false;  // it fits, but rows start on odd multiples of 16 bytes
+};
+TmaRows tma_rows(const at::Tensor& x) {
+    TmaRows r;
+    r.t = as_rows(x, &r.rows, &r.stride);
     const int64_t k = x.size(-1), e = x.element_size(), step = 16 / e;
-    if (*rows <= 1) *stride = (k + step - 1) / step * step;  // of no meaning for one row
-    if (reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 == 0 && *stride % step == 0 && *stride >= k) return r;
-    *stride = (k + step - 1) / step * step;
-    at::Tensor wide = at::empty({*rows, *stride}, x.options());
-    wide.narrow(1, 0, k).copy_(r.reshape({*rows, k}));
-    return wide;
+    if (r.rows <= 1) r.stride = (k + step - 1) / step * step;  // of no meaning for one row
+    const uintptr_t at = reinterpret_cast<uintptr_t>(r.t.data_ptr());
+    r.fits = at % 16 == 0 && r.stride % step == 0 && r.stride >= k;
+    r.slow = r.fits && r.rows > 1 && (at % 32 != 0 || r.stride % (2 * step) != 0);
+    return r;
+}
+
+// Copies an operand to rows a multiple of 128 bytes apart.
+void lay_out(TmaRows& r, void* stream) {
+    const int64_t k = r.t.size(-1), e = r.t.element_size(), step = 128 / e;
+    const int64_t stride = (k + step - 1) / step * step;
+    at::Tensor wide = at::empty({r.rows, stride}, r.t.options());
+    mindiesd_copy_rows_args c = {};
+    c.src = r.t.data_ptr();
+    c.dst = wide.data_ptr();
+    c.rows = r.rows;
+    c.row_bytes = k * e;
+    c.src_stride = r.stride * e;
+    c.dst_stride = stride * e;
+    check_rc(mindiesd_copy_rows(&c, stream), "mindiesd_copy_rows");
+    r.t = wide;
+    r.stride = stride;
+}
+
+// Lays out the operands that the kernel cannot take (an uneven width, a broadcast, an odd slice), and those that it takes
+// but fetches slowly where that pays.  A row that starts in the middle of a 32-byte sector costs the loads half again:
+// 5443 x 4376 x 12696 bf16 takes 755 us with both operands so, 594 with either one laid out by a copy (in the
+// time), 544 with both; 28213 x 2208 x 11848 takes 1240, 1071 with the weights laid out and 1309 with both, x being 668 MB.
+// The gain is a share of the product's time, a quarter for the operand with fewer rows where both are so, less for the
+// other; the copy moves its bytes twice at 6.5 TB/s.  Rows of less than 1.5 KB gain nothing, the epilogue
+// being what those products wait for (9197 x 10425 x 216 bf16: 209 us, and 209 on aligned rows).
+void lay_out_operands(TmaRows& x, TmaRows& w, bool fp8, void* stream) {
+    const int64_t k = x.t.size(-1), row_bytes = k * x.t.element_size();
+    const double product_us = 2.0 * static_cast<double>(x.rows) * static_cast<double>(w.rows) * static_cast<double>(k) / (fp8 ? 2.6e9 : 1.4e9);
+    const double last = fp8 ? 0.2 : 0.12;  // what the second of two, or the only one, gains
+    TmaRows& few = x.rows < w.rows ? x : w;
+    TmaRows& many = x.rows < w.rows ? w : x;
+    auto pays = [&](const TmaRows& r, double share) {
+        const double copy_us = 3.0 + 2.0 * static_cast<double>(r.rows) * static_cast<double>(row_bytes) / 6.5e6;
+        return r.slow && row_bytes >= 1536 && share * product_us > copy_us;
+    };
+    if (!few.fits || pays(few, many.slow ? 0.25 : last)) lay_out(few, stream);
+    if (!many.fits || pays(many, last)) lay_out(many, stream);
 }
 
 int activation_code(c10::string_view name) {
@@ -984,10 +1027,12 @@ at::Tensor linear_fwd_cuda(const at::Tensor& x, const at::Tensor& weight, const 
     const int act = activation_code(activation);
     if (m == 0) return out;
     c10::cuda::CUDAGuard guard(x.device());
-    int64_t rows_x = 0, rows_w = 0;
-    at::Tensor xr = as_tma_rows(x, &rows_x, &a.x_stride), wr = as_tma_rows(weight, &rows_w, &a.weight_stride);
-    a.x = xr.data_ptr();
-    a.weight = wr.data_ptr();
+    TmaRows xr = tma_rows(x), wr = tma_rows(weight);
+    lay_out_operands(xr, wr, fp8, stream_of(x));
+    a.x = xr.t.data_ptr();
+    a.weight = wr.t.data_ptr();
+    a.x_stride = xr.stride;
+    a.weight_stride = wr.stride;
     a.out = out.data_ptr();
     a.out_stride = n;
     a.m = static_cast<int32_t>(m);

@@ -166,6 +166,11 @@ class LinearArgs(C.Structure):
     ]
 
 
+class CopyRowsArgs(C.Structure):
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("rows", C.c_int64), ("row_bytes", C.c_int64),
+                ("src_stride", C.c_int64), ("dst_stride", C.c_int64)]
+
+
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 
 MAX_RANKS = 8
@@ -219,7 +224,8 @@ def lib():
         for name in ("mindiesd_attention_fwd", "mindiesd_rf_rearrange", "mindiesd_rf_block_mask",
                      "mindiesd_rf_pool", "mindiesd_rf_mask_from_pooled", "mindiesd_fa_block_quant",
                      "mindiesd_sparse_block_estimate", "mindiesd_fa_rotate_quant", "mindiesd_rope",
-                     "mindiesd_ulysses_move", "mindiesd_add_rms_norm", "mindiesd_linear_fwd"):
+                     "mindiesd_ulysses_move", "mindiesd_add_rms_norm", "mindiesd_linear_fwd",
+                     "mindiesd_copy_rows"):
             fn = getattr(handle, name, None)
             if fn is not None:
                 fn.restype = C.c_int

@@ -81,8 +81,8 @@ def linear_forward(x, weight, bias=None, activation="none", residual=None, gate=
     """out = residual + gate * act(x @ weight.T * x_scale * weight_scale + bias), accumulated and finished in fp32
     and rounded once.
 
-    x [..., K], weight [N, K]: both bf16, both fp16 or both e4m3.  Rows whose start and stride are multiples of 16
-    bytes are read in place; others are copied first.
+    x [..., K], weight [N, K]: both bf16, both fp16 or both e4m3.  Rows whose start and stride are multiples of 32
+    bytes are read in place; others are copied first (multiples of 16 bytes only where the copy is the shorter way).
     bias: [N], bf16, fp16 or fp32.  activation: "none", "relu", "silu", "gelu" (erf) or "gelu_tanh".
     gate: [N], or [B, N] / [B, 1, .., N] with B the first dimension of x; bf16, fp16 or fp32.
     residual: [..., N] in the output's type.

@@ -412,3 +412,82 @@ def test_failed_launch_leaves_no_error_behind():
     torch.cuda.synchronize()
     assert torch.count_nonzero(out).item() == 0
     _check(linear_forward(x, w), x, w, torch.bfloat16, 64)
+
+
+def test_copy_rows_refusals_without_a_gpu(tmp_path):
+    import shutil
+    import subprocess
+    from pathlib import Path
+    from mindiesd import _cabi
+    fn = _cabi.lib().mindiesd_copy_rows
+
+    def code(**changes):
+        a = _cabi.CopyRowsArgs(src=1 << 20, dst=2 << 20, rows=4, row_bytes=100, src_stride=100, dst_stride=128)
+        for name, value in changes.items():
+            setattr(a, name, value)
+        return fn(ctypes.byref(a), None)
+    assert fn(None, None) == -1 and code(src=None) == -1 and code(dst=None) == -1
+    assert code(rows=0) == -2 and code(row_bytes=0) == -2 and code(row_bytes=-1) == -2
+    assert code(rows=1 << 31) == -7 and code(row_bytes=1 << 34) == -7
+    assert code(rows=0x7fffffff, row_bytes=1 << 24, dst_stride=1 << 24) == -7  # more blocks than a grid has
+    assert code(src_stride=-100) == -4 and code(dst_stride=96) == -4 and code(dst_stride=120) == -4 and code(dst=(2 << 20) + 8) == -4
+    assert code(dst=(1 << 20) + 384) == -5 and code(src=(2 << 20) + 3 * 128 + 111) == -5  # they overlap by a byte
+    cc = shutil.which("gcc")
+    if cc:
+        src = tmp_path / "s.c"
+        src.write_text('#include <stdio.h>\n#include "mindiesd_b200.h"\nint main(void){printf("%zu",sizeof(mindiesd_copy_rows_args));return 0;}\n')
+        inc = Path(__file__).resolve().parent.parent / "include"
+        subprocess.run([cc, "-I", str(inc), str(src), "-o", str(tmp_path / "s")], check=True)
+        assert int(subprocess.run([str(tmp_path / "s")], capture_output=True, text=True, check=True).stdout) == ctypes.sizeof(_cabi.CopyRowsArgs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("row_bytes", [1, 2, 12, 40, 511, 512, 2048, 2064, 4098, 10001])
+@pytest.mark.parametrize("start,gap", [(0, 0), (1, 0), (2, 6), (4, 12), (8, 8), (16, 48)])
+def test_copy_rows(row_bytes, start, gap):
+    """Every width of piece, one segment of a row and several: the rows, zeros up to 16 bytes, and nothing behind."""
+    from mindiesd import _cabi
+    rows, stride, wide = 37, row_bytes + gap, (row_bytes + 15) // 16 * 16 + 32
+    buf = torch.randint(0, 256, (start + rows * stride,), dtype=torch.uint8, device="cuda")
+    src = buf[start:].view(rows, stride)[:, :row_bytes]
+    for step in (stride, 0):
+        dst = torch.full((rows + 1, wide), 7, dtype=torch.uint8, device="cuda")
+        a = _cabi.CopyRowsArgs(src.data_ptr(), dst.data_ptr(), rows, row_bytes, step, wide)
+        _cabi.check(_cabi.lib().mindiesd_copy_rows(ctypes.byref(a), _cabi.current_stream_ptr(dst.device)), "mindiesd_copy_rows")
+        assert torch.equal(dst[:rows, :row_bytes], src if step else src[:1].expand(rows, -1))
+        assert (dst[:rows, row_bytes:wide - 32] == 0).all() and (dst[:rows, wide - 32:] == 7).all() and (dst[rows] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("m,k,n", [(4096, 2056, 2100), (20000, 1544, 1536), (600, 4104, 9000), (300, 520, 400)])
+def test_rows_that_start_within_a_sector(m, k, n, dtype):
+    """Rows on odd multiples of 16 bytes, which are copied first where that pays: the same bits as on aligned rows, whichever
+    operand is so, on a stream of its own and replayed."""
+    from mindiesd import linear_forward
+    e = torch.empty(0, dtype=dtype).element_size()
+    k = k if e == 2 else k + 8
+    s = dict(x_scale=torch.full((1,), 0.5, device="cuda"), weight_scale=torch.full((1,), 2.0, device="cuda")) if e == 1 else {}
+
+    def at(t, stride):
+        wide = torch.zeros(t.shape[0], stride, dtype=torch.uint8, device="cuda").view(dtype)
+        wide[:, :t.shape[1]].copy_(t)
+        return wide[:, :t.shape[1]]
+    x, w = (_randn(seed, rows, k, scale=0.1).to(dtype) for seed, rows in ((110, m), (111, n)))
+    even, odd = (k * e + 127) // 128 * 128, (k * e + 127) // 128 * 128 + 16
+    xe, xo, we, wo = at(x, even), at(x, odd), at(w, even), at(w, odd)
+    want = linear_forward(xe, we, **s)
+    for a, b in ((xo, wo), (xo, we), (xe, wo), (x, w)):
+        assert torch.equal(linear_forward(a, b, **s), want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = [linear_forward(xo, wo, **s) for _ in range(3)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = linear_forward(xo, wo, **s)
+    xo.copy_(_randn(112, m, k, scale=0.1).to(dtype))
+    graph.replay()
+    assert torch.equal(captured, linear_forward(at(xo, even), we, **s))
