@@ -435,7 +435,7 @@ __global__ void __launch_bounds__(kRes > 0 ? 512 : 768) norm_stream_kernel(const
     }
 }
 
-// Rows that no 16-byte run fits: runs of four elements or single ones, straight from global memory, by blocks that
+// Rows that neither fit 16-byte runs nor lie side by side: runs of four elements or single ones, straight from global memory, by blocks that
 // stay.  A thread has the next row's runs on their way in registers while it works on the present row, and takes 16
 // elements of it, because a row's reduction costs every thread the same whatever its share (20000 x 1001 bf16: a
 // block of 256 threads per row, four elements each, issued 75 instructions per element and took 64 us).  kRes: 0 no residual, 1 in the type of x, 2 fp32.
@@ -508,6 +508,206 @@ __global__ void __launch_bounds__(512) norm_narrow_kernel(const NormParams p) {
 #pragma unroll
             for (int i = 0; i < kE; ++i) v[j][i] *= f;
             store_run<T, kE>(p, row * p.dim + at, v[j]);
+        }
+    }
+}
+
+// Stores elements [lo, hi) of a run, given as pairs of elements; at least one end is the run's own.
+template <typename P, int kPairs>
+__device__ __forceinline__ void store_part(P* at, const P (&v)[kPairs], int lo, int hi) {
+    using Half = std::conditional_t<sizeof(P) == 8, uint32_t, std::conditional_t<sizeof(P) == 4, uint16_t, uint8_t>>;
+    using Two = typename Raw<2 * sizeof(P)>::type;
+    constexpr int kE = 2 * kPairs;
+    union Twos {
+        P p[2];
+        Two two;
+        __device__ __forceinline__ Twos() {}
+    } t;
+    if (lo == 0 && hi == kE) {
+        if constexpr (kPairs * sizeof(P) <= 16) {
+            union {
+                P p[kPairs];
+                typename Raw<kPairs * sizeof(P)>::type all;
+            } u;
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) u.p[i] = v[i];
+            *reinterpret_cast<decltype(u.all)*>(at) = u.all;
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPairs; i += 2) {
+                t.p[0] = v[i];
+                t.p[1] = v[i + 1];
+                *reinterpret_cast<Two*>(at + i) = t.two;
+            }
+        }
+        return;
+    }
+    // A part of `count` elements is four, two and one of them, each on an address that its size divides.
+    const bool front = lo == 0;
+    const int count = front ? hi : kE - lo;
+    auto pick = [&](int q) {
+        P r = v[0];
+#pragma unroll
+        for (int i = 1; i < kPairs; ++i)
+            if (q == i) r = v[i];
+        return r;
+    };
+    if constexpr (kPairs == 4) {
+        if (count & 4) {
+            t.p[0] = front ? v[0] : v[2];
+            t.p[1] = front ? v[1] : v[3];
+            *reinterpret_cast<Two*>(at + (front ? 0 : 2)) = t.two;
+        }
+    }
+    if (count & 2) {
+        const int q = front ? (count & 4) / 2 : kPairs - 1 - (count & 4) / 2;
+        at[q] = pick(q);
+    }
+    if (count & 1) {
+        const int q = front ? count >> 1 : kPairs - 1 - (count >> 1);
+        const P pair = pick(q);
+        reinterpret_cast<Half*>(at)[2 * q + (front ? 0 : 1)] = static_cast<Half>(front ? pair : pair >> (4 * sizeof(P)));
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ auto pair_of(float lo, float hi) {
+    if constexpr (sizeof(T) == 4) return pack2(lo, hi);
+    else if constexpr (std::is_same_v<T, __half>) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+
+// Contiguous rows of a width that 16-byte runs do not divide.  The runs are those of the whole array, so a row starts
+// somewhere within its first one, and a run that two rows share is read by both and written in parts.  The weights, whose
+// place in a run differs from row to row, lie in shared memory as fp32, with a gap after every 32 for its banks.
+// Bound by instruction issue (bf16 with a residual 20000 x 1001 40 us, single elements 82, HBM 25; 6000 x 5121 54, 124, 38).
+__device__ __forceinline__ int banked(int i) { return i + (i >> 5); }
+
+template <int kE, typename W>
+__device__ __forceinline__ void stage_weights(float* to, const W* w, int dim) {
+    constexpr int kBatch = 8;  // loads on their way at once (one by one 5121 weights took 7 us)
+    for (int i0 = threadIdx.x; i0 < dim + 2 * kE; i0 += blockDim.x * kBatch) {
+        float v[kBatch];
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            const int i = i0 + b * blockDim.x - kE;
+            v[b] = i >= 0 && i < dim ? to_f32(w[i]) : 0.0f;
+        }
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            const int i = i0 + b * blockDim.x;
+            if (i < dim + 2 * kE) to[banked(i)] = v[b];
+        }
+    }
+}
+
+template <typename T, int kV, int kRes>
+__global__ void __launch_bounds__(512) norm_shifted_kernel(const NormParams p) {
+    using R = std::conditional_t<kRes == 2, float, T>;
+    constexpr int kE = 16 / sizeof(T);
+    extern __shared__ float weights[];  // [kE zeros | dim | kE zeros]
+    const int lane = threadIdx.x & (p.group - 1);
+    const int per_block = blockDim.x / p.group;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * per_block;
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * per_block + threadIdx.x / p.group;
+    const int64_t total = p.rows * p.dim;
+    const T* const x = static_cast<const T*>(p.x);
+    const R* const residual = static_cast<const R*>(p.residual);
+    auto shift_of = [&](int64_t row) { return (static_cast<int>(row) & (kE - 1)) * (p.dim & (kE - 1)) & (kE - 1); };
+    Run<T, kE> in[kV];
+    Run<R, kE> add[kV];
+    auto fetch = [&](int64_t row) {
+        if (row >= p.rows) return;
+        const int shift = shift_of(row);
+        const int64_t start = row * p.dim - shift;
+#pragma unroll
+        for (int j = 0; j < kV; ++j) {
+            const int c = (lane + j * p.group) * kE;
+            if (c - shift >= p.dim) continue;
+            if (start + c + kE <= total) {
+                in[j].load(x + start + c);
+                if constexpr (kRes > 0) add[j].load(residual + start + c);
+            } else {  // the array ends within this run
+#pragma unroll
+                for (int i = 0; i < kE; ++i)
+                    if (start + c + i < total) {
+                        in[j].d.elem[i] = x[start + c + i];
+                        if constexpr (kRes > 0) add[j].d.elem[i] = residual[start + c + i];
+                    }
+            }
+        }
+    };
+    allow_next_kernel();
+    wait_for_kernels_before();
+    fetch(first);
+    if (p.weight) {
+        if (p.weight_fp32) stage_weights<kE>(weights, static_cast<const float*>(p.weight), p.dim);
+        else stage_weights<kE>(weights, static_cast<const T*>(p.weight), p.dim);
+        __syncthreads();
+    }
+    int turn = 0;
+    for (int64_t row = first; row - threadIdx.x / p.group < p.rows; row += step) {
+        const bool live = row < p.rows;
+        const int shift = shift_of(row);
+        const int64_t start = row * p.dim - shift;
+        float v[kV][kE];
+#pragma unroll
+        for (int j = 0; j < kV; ++j) {
+#pragma unroll
+            for (int i = 0; i < kE; ++i) v[j][i] = kRes > 0 ? in[j].get(i) + add[j].get(i) : in[j].get(i);
+            const int at = (lane + j * p.group) * kE - shift;
+            if (at < 0 || at + kE > p.dim)
+#pragma unroll
+                for (int i = 0; i < kE; ++i)
+                    if (at + i < 0 || at + i >= p.dim) v[j][i] = 0.0f;
+        }
+        fetch(row + step);
+        Stats s = {0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < kV; ++j) {
+            const int at = (lane + j * p.group) * kE - shift;
+            if (!live || at >= p.dim) continue;
+            if constexpr (kRes > 0) {
+                decltype(pair_of<R>(0.0f, 0.0f)) pairs[kE / 2];
+#pragma unroll
+                for (int i = 0; i < kE / 2; ++i) pairs[i] = pair_of<R>(v[j][2 * i], v[j][2 * i + 1]);
+                store_part(reinterpret_cast<decltype(&pairs[0])>(static_cast<R*>(p.residual_out) + start + shift + at), pairs,
+                           max(0, -at), min(kE, p.dim - at));
+            }
+#pragma unroll
+            for (int i = 0; i < kE; ++i) {
+                s.sum += v[j][i] * v[j][i];
+                if (p.weight) v[j][i] *= weights[banked(at + kE + i)];
+                if (p.scales) s.top = max_nan(s.top, fabsf(v[j][i]));
+            }
+        }
+        s = p.scales ? reduce_row<true>(s, p.group, turn) : reduce_row<false>(s, p.group, turn);
+        turn ^= 1;
+        float scale = 1.0f;
+        const float f = row_factor(p, s, scale);
+        if (!live) continue;
+        if (p.scales && lane == 0) p.scales[row] = scale;
+#pragma unroll
+        for (int j = 0; j < kV; ++j) {
+            const int at = (lane + j * p.group) * kE - shift;
+            if (at >= p.dim) continue;
+            const int lo = max(0, -at), hi = min(kE, p.dim - at);
+            if (p.scales) {
+                uint16_t pairs[kE / 2];
+#pragma unroll
+                for (int i = 0; i < kE / 2; ++i) pairs[i] = e4m3x2(v[j][2 * i] * f, v[j][2 * i + 1] * f);
+                store_part(reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(p.out) + start + shift + at), pairs, lo, hi);
+            } else {
+                decltype(pair_of<T>(0.0f, 0.0f)) pairs[kE / 2];
+#pragma unroll
+                for (int i = 0; i < kE / 2; ++i) pairs[i] = pair_of<T>(v[j][2 * i] * f, v[j][2 * i + 1] * f);
+                store_part(reinterpret_cast<decltype(&pairs[0])>(static_cast<T*>(p.out) + start + shift + at), pairs, lo, hi);
+            }
         }
     }
 }
@@ -632,6 +832,32 @@ cudaError_t launch_narrow(const NormParams& p, int threads, cudaStream_t stream)
     return launch(norm_narrow_kernel<T, kE, kV, 2>, p, grid, threads, 0, stream);
 }
 
+template <typename T, int kV>
+cudaError_t launch_shifted(const NormParams& p, int threads, int smem, cudaStream_t stream) {
+    const int64_t blocks = (p.rows + threads / p.group - 1) / (threads / p.group);
+    const int64_t grid = std::min<int64_t>(blocks, kSms * (1024 / threads));
+    if (!p.residual) return launch(norm_shifted_kernel<T, kV, 0>, p, grid, threads, smem, stream);
+    if (!p.residual_fp32) return launch(norm_shifted_kernel<T, kV, 1>, p, grid, threads, smem, stream);
+    return launch(norm_shifted_kernel<T, kV, 2>, p, grid, threads, smem, stream);
+}
+
+constexpr int kShiftedMost = 3;         // runs of a thread
+constexpr int kShiftedMaxDim = 11000;   // the weights in 48 KB of shared memory
+
+template <typename T>
+cudaError_t launch_shifted(NormParams p, cudaStream_t stream) {
+    constexpr int kE = 16 / sizeof(T);
+    const int runs = (p.dim + 2 * kE - 2) / kE;  // of a row that starts on the last element of one
+    p.group = 1;
+    while (p.group < 512 && p.group * kShiftedMost < runs) p.group *= 2;
+    const int threads = std::max(p.group, 128), smem = p.weight ? (p.dim + 2 * kE) / 32 * 132 + 132 : 0;
+    switch ((runs + p.group - 1) / p.group) {
+        case 1: return launch_shifted<T, 1>(p, threads, smem, stream);
+        case 2: return launch_shifted<T, 2>(p, threads, smem, stream);
+        default: return launch_shifted<T, kShiftedMost>(p, threads, smem, stream);
+    }
+}
+
 template <typename T, int kE>
 cudaError_t launch_rows(NormParams p, cudaStream_t stream) {
     const int runs = (p.dim + kE - 1) / kE;
@@ -687,10 +913,18 @@ cudaError_t launch_typed(const NormParams& p, cudaStream_t stream) {
                rows_at(p.residual_out, p.dim, re, run) && rows_at(p.weight, 0, p.weight_fp32 ? 4 : e, run) &&
                rows_at(p.out, p.dim, oe, run);
     };
-    if constexpr (sizeof(T) == 2) {
-        if (fits(8)) return launch_rows<T, 8>(p, stream);
+    constexpr int kWide = 16 / sizeof(T);
+    if (fits(kWide)) return launch_rows<T, kWide>(p, stream);
+    auto starts = [](const void* base, int bytes) { return reinterpret_cast<uintptr_t>(base) % bytes == 0; };
+    const bool packed = (p.rows == 1 || (p.x_stride == p.dim && (!p.residual || p.residual_stride == p.dim))) && starts(p.x, 16) &&
+                        starts(p.residual, 16) && starts(p.residual_out, 16) && starts(p.out, p.scales ? kWide : 16);
+    // Runs of half the width suit rows that they divide, as long as no residual adds to the loads or the rows are short
+    // (bf16, half / shared whole ones: 20000 x 1004 20 / 27 us, with a residual 34 / 40; 10000 x 1500 19 / 22 and 31 / 28;
+    // 6000 x 5124 42 / 44 and 66 / 53).
+    if constexpr (kWide == 8) {
+        if (fits(4) && (!p.residual || p.dim <= 1024 || !packed)) return launch_rows<T, 4>(p, stream);
     }
-    if (fits(4)) return launch_rows<T, 4>(p, stream);
+    if (packed && p.dim >= kWide && p.dim <= kShiftedMaxDim && p.dim <= kWide * (512 * kShiftedMost - 2)) return launch_shifted<T>(p, stream);
     return launch_rows<T, 1>(p, stream);
 }
 

@@ -318,3 +318,65 @@ def test_streams_graphs_and_repeatability():
     torch.cuda.synchronize()
     for a, b in zip(captured, add_rms_norm_quant(x, None, r)):
         assert torch.equal(a.float(), b.float())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("dim", [5, 9, 15, 18, 98, 100, 179, 514, 1003, 1004, 4097, 6143, 10999, 11002])
+def test_packed_rows_of_uneven_width(dim, dtype):
+    """Rows that start anywhere in a 16-byte run and share runs with their neighbours: the values, the last row at the very
+    end of its memory, and neighbours of a NaN as if it were not there.  Rows apart from one another agree."""
+    from mindiesd import add_rms_norm, add_rms_norm_quant
+    for rows, weight, residual in [(1, dtype, dtype), (2, None, torch.float32), (45, torch.float32, None), (4003, dtype, dtype),
+                                   (3001, None, torch.float32)]:
+        x = _randn(dim + rows, rows, dim, dtype=dtype)
+        w = None if weight is None else _randn(1, dim, dtype=weight)
+        r = None if residual is None else _randn(2, rows, dim, dtype=residual, scale=3.0)
+        keep = torch.ones(rows, dtype=torch.bool, device="cuda")
+        if rows > 2:
+            x[rows // 2, 0] = x[rows // 3, dim - 1] = float("nan")
+            keep[rows // 2] = keep[rows // 3] = False
+        y64, v64 = ob.rms_norm(x, w, r)
+        got, quant = add_rms_norm(x, w, r), add_rms_norm_quant(x, w, r)
+        if r is not None:
+            got, total = got
+            assert torch.equal(quant[2].nan_to_num(), total.nan_to_num()) and torch.equal(total.isnan(), v64.isnan())
+            _close(total.nan_to_num(), v64.nan_to_num(), residual)
+        assert got[~keep].isnan().all() and quant[1][~keep].isnan().all()
+        _close(got[keep], y64[keep], dtype)
+        _close_quant(quant[0][keep], quant[1][keep], y64[keep])
+        # the same rows lying apart take another kernel, whose sums run in another order
+        wide = torch.zeros(rows, dim + 3, dtype=dtype, device="cuda")[:, :dim].copy_(x)
+        apart = add_rms_norm(wide, w, r)
+        _close((apart if r is None else apart[0])[keep], y64[keep], dtype)
+
+
+@pytest.mark.gpu
+def test_packed_rows_of_uneven_width_write_nothing_else():
+    """Through the C ABI: what lies before and behind the outputs stays, at every position of the last element in a run."""
+    from mindiesd import _cabi
+    for dim in range(33, 42):
+        for rows in (1, 2, 7):
+            x, r = _randn(1, rows, dim, dtype=torch.bfloat16), _randn(2, rows, dim, dtype=torch.float32)
+            w = _randn(3, dim, dtype=torch.bfloat16)
+            for e4m3 in (False, True):
+                buf = torch.full((rows * dim + 64,), 7.0, device="cuda").to(torch.float8_e4m3fn if e4m3 else torch.bfloat16)
+                total, scales = torch.full((rows * dim + 64,), 7.0, device="cuda"), torch.full((rows + 2,), 7.0, device="cuda")
+                a = _cabi.NormArgs()
+                a.x, a.residual, a.weight = x.data_ptr(), r.data_ptr(), w.data_ptr()
+                a.out, a.residual_out = buf[32:].data_ptr(), total[32:].data_ptr()
+                a.scales = scales[1:].data_ptr() if e4m3 else None
+                a.rows, a.dim, a.x_stride, a.residual_stride, a.eps = rows, dim, dim, dim, 1e-6
+                a.dtype = a.weight_dtype = _cabi.BF16
+                a.residual_dtype, a.out_dtype = _cabi.FP32, _cabi.E4M3 if e4m3 else _cabi.BF16
+                _cabi.check(_cabi.lib().mindiesd_add_rms_norm(ctypes.byref(a), _cabi.current_stream_ptr(x.device)), "mindiesd_add_rms_norm")
+                y64, v64 = ob.rms_norm(x, w, r)
+                n = rows * dim
+                _close(total[32:32 + n].view(rows, dim), v64, torch.float32)
+                if e4m3:
+                    _close_quant(buf[32:32 + n].view(rows, dim), scales[1:-1, None], y64)
+                    assert scales[0] == 7 and scales[-1] == 7
+                else:
+                    _close(buf[32:32 + n].view(rows, dim), y64, torch.bfloat16)
+                for t in (buf.float(), total):
+                    assert (t[:32] == 7).all() and (t[32 + n:] == 7).all()
