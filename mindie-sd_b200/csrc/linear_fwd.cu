@@ -43,7 +43,8 @@ struct Epilogue {
     int x_scale_step, w_scale_step;  // 0: one scale for all
     int bias_type, gate_type;        // MINDIESD_BF16 / FP16 / FP32
     int out_fp16, act;
-    int wide_out, wide_residual, wide_gate;  // rows can be moved 16 bytes at a time
+    int out_piece, residual_piece;   // bytes of a row that can be moved at a time (piece_of)
+    int wide_gate;                   // 16 of them
     int m, n;
 };
 
@@ -208,7 +209,7 @@ static_assert(kPairSmem <= 227 * 1024, "shared memory of the pair kernel");
 // the piece-wise reads free of bank conflicts.
 __device__ __forceinline__ uint32_t staged(int r, int c) { return r * 32 + ((c ^ ((r >> 2) & 1)) << 4); }
 
-// A lane's share of a unit in a two-byte row-major matrix: 8 columns of rows lane/2 and lane/2 + 16 of the warp's 32.
+// A lane's share of a unit on its way through the staging buffer: 8 columns of rows lane/2 and lane/2 + 16 of the warp's 32.
 struct UnitAt {
     const uint16_t* p[2];
     bool live[2];  // the rows exist
@@ -222,32 +223,82 @@ struct UnitAt {
     }
 };
 
-__device__ __forceinline__ void fetch_unit(uint4 (&v)[2], const UnitAt& at, int col0, int n, bool wide, int lane) {
+// 32 bytes of a row that starts on a multiple of 32.
+__device__ __forceinline__ void load_row32(uint32_t (&w)[8], const uint16_t* p) {
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                 : "l"(p)
+                 : "memory");
+}
+__device__ __forceinline__ void store_row32(uint16_t* p, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+
+// `piece`: 16 or 8 bytes where every row starts on a multiple of that and holds whole ones, else 2.  Rows of an odd
+// width start on 4 bytes and between them in turn; the words of the latter are shifted by one element.
+__device__ __forceinline__ void fetch_unit(uint32_t (&words)[8], const UnitAt& at, int col0, int n, int piece, int lane) {
     const int left = n - col0 - (lane & 1) * 8;  // columns of this lane that exist
+    uint4 v[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        v[i] = make_uint4(0, 0, 0, 0);
         if (!at.live[i] || left <= 0) continue;
-        if (wide) {
-            v[i] = __ldg(reinterpret_cast<const uint4*>(at.p[i] + col0));
+        const uint16_t* p = at.p[i] + col0;
+        if (piece == 16) {
+            v[i] = __ldg(reinterpret_cast<const uint4*>(p));
+        } else if (piece == 8) {
+            const uint2 lo = __ldg(reinterpret_cast<const uint2*>(p));
+            const uint2 hi = left > 4 ? __ldg(reinterpret_cast<const uint2*>(p) + 1) : make_uint2(0, 0);
+            v[i] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        } else if (left >= 8) {
+            const bool odd = reinterpret_cast<uintptr_t>(p) & 2;
+            const uint32_t* q = reinterpret_cast<const uint32_t*>(p + odd);
+            const uint32_t a = __ldg(q), b = __ldg(q + 1), c = __ldg(q + 2);
+            if (odd) {
+                const uint32_t first = __ldg(p), last = __ldg(p + 7);
+                v[i] = make_uint4(first | (a << 16), (a >> 16) | (b << 16), (b >> 16) | (c << 16), (c >> 16) | (last << 16));
+            } else {
+                v[i] = make_uint4(a, b, c, __ldg(q + 3));
+            }
         } else {
             uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (j < left) w[j >> 1] |= static_cast<uint32_t>(at.p[i][col0 + j]) << ((j & 1) * 16);
+                if (j < left) w[j >> 1] |= static_cast<uint32_t>(p[j]) << ((j & 1) * 16);
             v[i] = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
-}
-__device__ __forceinline__ void put_unit(char* buf, const uint4 (&v)[2], int lane) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) *reinterpret_cast<uint4*>(buf + staged(i * 16 + (lane >> 1), lane & 1)) = v[i];
+    for (int i = 0; i < 2; ++i) {
+        words[4 * i] = v[i].x;
+        words[4 * i + 1] = v[i].y;
+        words[4 * i + 2] = v[i].z;
+        words[4 * i + 3] = v[i].w;
+    }
+}
+// Turns what fetch_unit loaded into this lane's row of the unit, through the warp's staging buffer.
+__device__ __forceinline__ void turn_unit(char* buf, uint32_t (&w)[8], int lane) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        *reinterpret_cast<uint4*>(buf + staged(i * 16 + (lane >> 1), lane & 1)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    __syncwarp();
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const uint4 v = *reinterpret_cast<const uint4*>(buf + staged(lane, q));
+        w[4 * q] = v.x;
+        w[4 * q + 1] = v.y;
+        w[4 * q + 2] = v.z;
+        w[4 * q + 3] = v.w;
+    }
+    __syncwarp();
 }
 
-// Writes a warp's staging buffer to the output: 16 rows of 32 bytes at a time, or two rows of 16 elements where 16-byte
-// access is not possible.
+// Writes a warp's staging buffer to the output where the rows' pieces are smaller than 32 bytes: 16 rows of 32 bytes at a time,
+// or fewer rows in smaller pieces (9000 x 256 x n bf16, single elements 94 us: n 5128 55 us, 5124 60 in pieces of 8 bytes,
+// 5122 84 and 5121 92 in words; 5120, where a lane stores its own 32 bytes, 46, and 52 through this buffer).
 __device__ __forceinline__ void stage_out(const char* buf, const UnitAt& at, const Epilogue& e, int row0, int col0, int lane) {
-    if (e.wide_out) {
+    if (e.out_piece == 16) {
         if (col0 + (lane & 1) * 8 < e.n) {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
@@ -255,14 +306,44 @@ __device__ __forceinline__ void stage_out(const char* buf, const UnitAt& at, con
                     *reinterpret_cast<uint4*>(const_cast<uint16_t*>(at.p[i]) + col0) =
                         *reinterpret_cast<const uint4*>(buf + staged(i * 16 + (lane >> 1), lane & 1));
         }
+        return;
+    }
+    uint16_t* const g = static_cast<uint16_t*>(e.out) + static_cast<int64_t>(row0) * e.out_stride + col0;
+    if (e.out_piece == 8) {
+        const int c = (lane & 3) * 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = i * 8 + (lane >> 2);
+            if (row0 + r < e.m && col0 + c < e.n)
+                *reinterpret_cast<uint2*>(g + r * e.out_stride + c) = *reinterpret_cast<const uint2*>(buf + staged(r, c >> 3) + (c & 4) * 2);
+        }
+    } else if (col0 + kUnit <= e.n) {
+        // Word c of every fourth row: whether its rows start between words does not change from one to the next.
+        const int c = lane & 7, r0 = lane >> 3, c1 = (c + 1) & 7;
+        uint16_t* p = g + r0 * e.out_stride + c * 2;
+        const uint32_t odd = (reinterpret_cast<uintptr_t>(p) & 2) / 2;
+        p += odd;
+        const int live = c == 7 && odd ? 0 : e.m - row0 - r0;  // rows of this lane lie below it
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const char* row = buf + i * 128 + r0 * 32;
+            const uint32_t lo = *reinterpret_cast<const uint32_t*>(row + ((((c >> 2) ^ i) & 1) << 4) + (c & 3) * 4);
+            const uint32_t hi = *reinterpret_cast<const uint32_t*>(row + ((((c1 >> 2) ^ i) & 1) << 4) + (c1 & 3) * 4);
+            if (i * 4 < live) *reinterpret_cast<uint32_t*>(p) = __funnelshift_r(lo, hi, odd * 16);
+            p += 4 * e.out_stride;
+        }
+        uint16_t* ends = g + lane * e.out_stride;
+        if (row0 + lane < e.m && (reinterpret_cast<uintptr_t>(ends) & 2)) {  // what the words leave of such a row
+            ends[0] = *reinterpret_cast<const uint16_t*>(buf + staged(lane, 0));
+            ends[15] = *reinterpret_cast<const uint16_t*>(buf + staged(lane, 1) + 14);
+        }
     } else {
         const int c = lane & 15;
-        uint16_t* g = static_cast<uint16_t*>(e.out) + static_cast<int64_t>(row0) * e.out_stride + col0 + c;
 #pragma unroll 4
         for (int i = 0; i < 16; ++i) {
             const int r = i * 2 + (lane >> 4);
             if (row0 + r < e.m && col0 + c < e.n)
-                g[r * e.out_stride] = *reinterpret_cast<const uint16_t*>(buf + staged(r, c >> 3) + (c & 7) * 2);
+                g[r * e.out_stride + c] = *reinterpret_cast<const uint16_t*>(buf + staged(r, c >> 3) + (c & 7) * 2);
         }
     }
 }
@@ -425,7 +506,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
         float* cols = reinterpret_cast<float*>(columns + (warp - 4) * kColsBytes);  // [bias | weight scale | gate][kCols]
         const uint32_t acc_empty0 = cluster_map(acc_empty, 0);
         const uint16_t* residual = static_cast<const uint16_t*>(e.residual);
-        uint4 ahead[2];  // the residual of the next unit
+        uint32_t ahead[kUnit / 2];  // the residual of the next unit: of this lane's row, or to be passed through shared memory
         int acc = 0;
         uint32_t acc_phase = 0;
         bool ok = !gave_up_before;
@@ -464,8 +545,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
                 for (int u = turn; u < units; u += kUnitWarps)
                     prefetch_l2(residual + static_cast<int64_t>(row) * e.residual_stride + min(tn * p.tile_n + u * kUnit, e.n - 1));
             __syncwarp();
+            uint16_t* const out_row = static_cast<uint16_t*>(e.out) + static_cast<int64_t>(row) * e.out_stride;
             // Values of a unit's columns in this lane's row (the j-th unit of the warp), from accumulator to output.
-            auto finish = [&](uint64_t (&v)[kUnit / 2], int j, int col0) {
+            auto finish = [&](uint64_t (&v)[kUnit / 2], const uint32_t (&old)[kUnit / 2], int j, int col0) {
                 const ulonglong2* at = reinterpret_cast<const ulonglong2*>(cols + j * kUnit);  // two pairs of columns per load
                 if constexpr (kFp8) {
 #pragma unroll
@@ -502,21 +584,19 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
                 }
                 if (e.residual) {
 #pragma unroll
-                    for (int q = 0; q < kUnit / 8; ++q) {
-                        const uint4 old = *reinterpret_cast<const uint4*>(buf + staged(lane, q));
-                        const uint32_t w[4] = {old.x, old.y, old.z, old.w};
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            float lo, hi;
-                            unpack_pair(w[i], e.out_fp16, lo, hi);
-                            v[q * 4 + i] = add2(v[q * 4 + i], pack2(lo, hi));
-                        }
+                    for (int i = 0; i < kUnit / 2; ++i) {
+                        float lo, hi;
+                        unpack_pair(old[i], e.out_fp16, lo, hi);
+                        v[i] = add2(v[i], pack2(lo, hi));
                     }
-                    __syncwarp();
                 }
                 uint32_t w[kUnit / 2];
                 if (e.out_fp16) pack_values<true>(v, w);
                 else pack_values<false>(v, w);
+                if (e.out_piece == 32) {
+                    if (live && col0 < e.n) store_row32(out_row + col0, w);
+                    return;
+                }
 #pragma unroll
                 for (int q = 0; q < kUnit / 8; ++q)
                     *reinterpret_cast<uint4*>(buf + staged(lane, q)) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
@@ -526,7 +606,15 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
             };
             const uint32_t tmem_rows = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
             const float nan = __uint_as_float(0x7fc00000u);  // what a wait that gave up leaves: never plausible numbers
-            if (e.residual) fetch_unit(ahead, residual_at, tn * p.tile_n + turn * kUnit, e.n, e.wide_residual, lane);
+            const uint16_t* const residual_row = residual + static_cast<int64_t>(row) * e.residual_stride;
+            auto fetch = [&](int col0) {
+                if (e.residual_piece == 32) {
+                    if (live && col0 < e.n) load_row32(ahead, residual_row + col0);
+                } else {
+                    fetch_unit(ahead, residual_at, col0, e.n, e.residual_piece, lane);
+                }
+            };
+            if (e.residual) fetch(tn * p.tile_n + turn * kUnit);
             // The first tile starts with a pass beyond the last column, which loads and stores nothing: it brings
             // the code below into the instruction cache while the first MMAs run.
 #pragma unroll 1
@@ -551,13 +639,14 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
                     for (int i = 0; i < kUnit / 2; ++i) v[i] = pack2(__uint_as_float(bits[2 * i]), __uint_as_float(bits[2 * i + 1]));
                 }
                 if (col0 >= e.n && j >= 0) continue;
+                uint32_t old[kUnit / 2] = {};
                 if (e.residual && j >= 0) {
-                    put_unit(buf, ahead, lane);
-                    __syncwarp();
-                    if (u + kUnitWarps < units)
-                        fetch_unit(ahead, residual_at, col0 + kUnitWarps * kUnit, e.n, e.wide_residual, lane);
+                    if (e.residual_piece != 32) turn_unit(buf, ahead, lane);
+#pragma unroll
+                    for (int i = 0; i < kUnit / 2; ++i) old[i] = ahead[i];
+                    if (u + kUnitWarps < units) fetch(col0 + kUnitWarps * kUnit);
                 }
-                finish(v, j < 0 ? 0 : j, col0);
+                finish(v, old, j < 0 ? 0 : j, col0);
             }
             if (units <= turn) {  // a tile with fewer units than warps: this one only hands the accumulator back
                 if (ok) ok = mbar_wait(acc_full + 8 * acc, acc_phase, abort_flag, 5, limit);
@@ -653,7 +742,7 @@ __global__ void __launch_bounds__(kSwapThreads) linear_swap_kernel(const __grid_
         }
         const uint32_t lo = pack_pair(v[0], v[1], e.out_fp16), hi = pack_pair(v[2], v[3], e.out_fp16);
         uint16_t* o = static_cast<uint16_t*>(e.out) + row * e.out_stride + first;
-        if (e.wide_out) {  // n is a multiple of 8 then
+        if (e.out_piece >= 8) {  // n is a multiple of 4 then
             if (first < e.n) *reinterpret_cast<uint2*>(o) = make_uint2(lo, hi);
         } else {
 #pragma unroll
@@ -1062,9 +1151,13 @@ extern "C" int mindiesd_linear_fwd(const mindiesd_linear_args* a, void* stream_)
     e.act = a->activation;
     e.m = a->m;
     e.n = a->n;
-    // 16-byte access: rows start on a 16-byte boundary and hold whole vectors.
-    e.wide_out = aligned(a->out, 16) && e.out_stride % 8 == 0 && a->n % 8 == 0;
-    e.wide_residual = a->residual && aligned(a->residual, 16) && a->residual_stride % 8 == 0 && a->n % 8 == 0;
+    // The largest piece that every row starts on and holds a whole number of.
+    auto piece_of = [&](const void* ptr, int64_t stride) {
+        const uintptr_t bits = reinterpret_cast<uintptr_t>(ptr) | static_cast<uintptr_t>(stride) * 2 | static_cast<uintptr_t>(a->n) * 2;
+        return bits % 32 == 0 ? 32 : bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : 2;
+    };
+    e.out_piece = piece_of(a->out, e.out_stride);
+    e.residual_piece = a->residual ? piece_of(a->residual, a->residual_stride) : 32;
     e.wide_gate = a->gate && aligned(a->gate, 16) && (a->gate_stride * dtype_bytes(a->gate_dtype)) % 16 == 0;
     p.wait_limit_us = a->wait_limit_us ? a->wait_limit_us : kWaitLimitUs;
     p.test_withhold = a->test_withhold;

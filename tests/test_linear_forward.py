@@ -491,3 +491,29 @@ def test_rows_that_start_within_a_sector(m, k, n, dtype):
     xo.copy_(_randn(112, m, k, scale=0.1).to(dtype))
     graph.replay()
     assert torch.equal(captured, linear_forward(at(xo, even), we, **s))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [256, 264, 260, 258, 257, 287])
+def test_rows_of_every_piece(n, dtype):
+    """Outputs and residuals whose rows can be moved 32, 16, 8 or 4 bytes at a time, or start between words in turn, each
+    with the other on an address of its own; what surrounds the output stays."""
+    from mindiesd import _cabi
+    m, k = 4400, 64
+    x, w, _ = _operands(120, m, k, n, dtype)
+    for out_start, out_pad, res_start, res_pad in ((0, 0, 0, 0), (16, 32, 0, 16), (8, 8, 4, 4), (4, 4, 2, 2), (2, 2, 1, 1), (1, 1, 0, 3), (1, 16, 16, 16)):
+        wide = torch.full((m + 2, n + out_pad + out_start), 7.0, dtype=dtype, device="cuda")
+        out = wide[1:1 + m, out_start:out_start + n]
+        r = _randn(121, m, n + res_pad + res_start, dtype=dtype)[:, res_start:res_start + n]
+        a = _cabi.LinearArgs()
+        a.x, a.weight, a.out, a.residual = x.data_ptr(), w.data_ptr(), out.data_ptr(), r.data_ptr()
+        a.x_stride = a.weight_stride = k
+        a.out_stride, a.residual_stride = wide.stride(0), r.stride(0)
+        a.m, a.n, a.k = m, n, k
+        a.in_dtype = a.out_dtype = _cabi.dtype_code(dtype)
+        _cabi.check(_cabi.lib().mindiesd_linear_fwd(ctypes.byref(a), _cabi.current_stream_ptr(x.device)), "mindiesd_linear_fwd")
+        _check(out, x, w, dtype, k, residual=r)
+        keep = torch.ones_like(wide, dtype=torch.bool)
+        keep[1:1 + m, out_start:out_start + n] = False
+        assert (wide[keep] == 7).all()
