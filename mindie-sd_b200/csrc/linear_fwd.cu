@@ -138,11 +138,27 @@ __device__ __forceinline__ uint64_t over_one_plus_ex2(uint64_t v, uint64_t x) {
     return mul2(v, pack2(rcp_approx(lo), rcp_approx(hi)));
 }
 
-// Out of line: 32 copies of erfc in the epilogue's loop cost registers that the other activations need.
-__device__ __noinline__ float gelu_erf(float v) { return 0.5f * v * erfcf(-0.70710678118654752f * v); }
+// gelu(v) = max(v, 0) - |v|/2 erfc(|v| / sqrt 2), which loses nothing for large negative v, for a pair of values.  With
+// z = |v| / sqrt 2 and t = 1 / (1 + 0.45 z), erfc(z) = e^(-z^2) t P(t); P is the polynomial of degree 7 with the smallest
+// largest relative error (3.5e-7) for z up to 14.2, found by linear programming.  Beyond, the product is 0.
+// (CUDA's erfc, out of line: 9000 x 1024 x 5120 bf16 150 us, this 85, gelu_tanh 79; 9000 x 5120 x 5120 321 and 307.)
+__device__ __forceinline__ uint64_t gelu_pair(uint64_t v) {
+    constexpr float kP[8] = {0.253884882f, 0.254008859f, 0.225756422f, 0.196237445f, 0.0261506569f, 0.223944306f, -0.248876333f, 0.0688941106f};
+    float lo, hi, x, y;
+    unpack2(v, lo, hi);
+    const uint64_t a = pack2(fminf(fabsf(lo), 20.0f), fminf(fabsf(hi), 20.0f));  // an infinity would give 0 * infinity
+    unpack2(fma2(a, both(0.45f * 0.70710678f), both(1.0f)), x, y);
+    const uint64_t t = pack2(rcp_approx(x), rcp_approx(y));
+    uint64_t q = both(kP[7]);
+#pragma unroll
+    for (int i = 6; i >= 0; --i) q = fma2(q, t, both(kP[i]));
+    unpack2(mul2(mul2(a, a), both(-0.5f * 1.4426950408889634f)), x, y);
+    q = mul2(mul2(q, t), pack2(ex2_approx(x), ex2_approx(y)));
+    return fma2(mul2(a, both(-0.5f)), q, pack2(lo < 0.0f ? 0.0f : lo, hi < 0.0f ? 0.0f : hi));  // a NaN stays
+}
 
 // The activations, on pairs of values, in the forms that keep their relative accuracy for large negative arguments:
-//   gelu(v) = v/2 erfc(-v / sqrt 2),  silu(v) = v / (1 + e^-v),
+//   gelu(v) = v/2 erfc(-v / sqrt 2) (gelu_pair),  silu(v) = v / (1 + e^-v),
 //   gelu_tanh(v) = v/2 (1 + tanh u) = v / (1 + e^-2u),  u = sqrt(2/pi) (v + 0.044715 v^3).
 template <int kPairs>
 __device__ __forceinline__ void activate(uint64_t (&v)[kPairs], int act) {
@@ -163,11 +179,7 @@ __device__ __forceinline__ void activate(uint64_t (&v)[kPairs], int act) {
             break;
         case kGelu:
 #pragma unroll
-            for (int i = 0; i < kPairs; ++i) {
-                float lo, hi;
-                unpack2(v[i], lo, hi);
-                v[i] = pack2(gelu_erf(lo), gelu_erf(hi));
-            }
+            for (int i = 0; i < kPairs; ++i) v[i] = gelu_pair(v[i]);
             break;
         case kGeluTanh:
 #pragma unroll

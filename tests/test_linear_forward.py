@@ -517,3 +517,23 @@ def test_rows_of_every_piece(n, dtype):
         keep = torch.ones_like(wide, dtype=torch.bool)
         keep[1:1 + m, out_start:out_start + n] = False
         assert (wide[keep] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["relu", "silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("m", [3, 700])
+def test_activations_over_their_range(act, m):
+    """One product per value (the other operand is the unit matrix), so the activation's own error shows: a fine sweep of
+    both signs, the largest arguments, and what must come of an infinity and a NaN."""
+    from mindiesd import linear_forward
+    n = 128
+    eye = torch.eye(n, dtype=torch.bfloat16, device="cuda")
+    values = torch.cat([torch.linspace(-14, 14, m * n - 40, device="cuda"), torch.logspace(-30, 3, 20, device="cuda"),
+                        -torch.logspace(-30, 3, 20, device="cuda")]).to(torch.bfloat16).view(m, n)
+    _check(linear_forward(values, eye, activation=act), values, eye, torch.bfloat16, n, act=act)
+    x = torch.zeros(m, n, dtype=torch.bfloat16, device="cuda")
+    bias = torch.zeros(n, device="cuda")
+    bias[1], bias[2], bias[5] = float("inf"), float("nan"), -40.0
+    y = linear_forward(x, eye, bias, activation=act)
+    assert (y[:, 1] == float("inf")).all() and y[:, 2].isnan().all()
+    assert (y[:, 5].float().abs() < 1e-15).all() and (y[:, [0, 3, 4, 6]] == 0).all()
