@@ -21,6 +21,7 @@ namespace {
 
 constexpr float kE4m3Max = 448.0f;
 constexpr float kMinScale = 1.17549435e-38f;  // 2^-126: below it 1 / scale would overflow
+constexpr float kMaxFloat = 3.40282347e38f;   // what is above it is infinite
 
 struct NormParams {
     const void* x;
@@ -73,13 +74,21 @@ __device__ __forceinline__ void store_global32(float* p, const float (&v)[8]) {
                  : "memory");
 }
 
-// Factors that turn v * w into the stored value, from the row's statistics.
-__device__ __forceinline__ float row_factor(const NormParams& p, const Stats& s, float& scale) {
+// What turns v * w into the stored value, from the row's statistics: v * w * first * second.
+struct Factors {
+    float first, second;
+};
+
+// For e4m3 the two factors are rstd and 1 / scale.  Each is finite (eps > 0, scale >= 2^-126), but their product, 448 / max|v w|
+// unless the scale is at its lower bound, overflows for rows of values below 1.4e-36: only there the values take them one after the
+// other, everywhere else their product alone.
+__device__ __forceinline__ Factors row_factors(const NormParams& p, const Stats& s, float& scale) {
     const float rstd = p.norm ? rsqrtf(s.sum * p.inv_dim + p.eps) : 1.0f;
-    if (!p.scales) return rstd;
+    if (!p.scales) return {1.0f, rstd};
     const float top = s.top * rstd;
     scale = top == 0.0f ? 1.0f : max_nan(top / kE4m3Max, kMinScale);
-    return rstd * (1.0f / scale);
+    const float inverse = 1.0f / scale, both = rstd * inverse;
+    return both > kMaxFloat ? Factors{rstd, inverse} : Factors{1.0f, both};
 }
 
 template <typename T, int kE>
@@ -201,15 +210,18 @@ __global__ void __launch_bounds__(1024) norm_row_kernel(const NormParams p) {
     }
     s = reduce_row<true>(s, p.group);
     float scale = 1.0f;
-    const float f = row_factor(p, s, scale);
+    const Factors f = row_factors(p, s, scale);
     if (!live) return;
     if (p.scales && lane == 0) p.scales[row] = scale;
 #pragma unroll
     for (int j = 0; j < kV; ++j) {
         const int at = (lane + j * p.group) * kE;
         if (at >= p.dim) continue;
+        if (f.first != 1.0f)
 #pragma unroll
-        for (int i = 0; i < kE; ++i) v[j][i] *= f;
+            for (int i = 0; i < kE; ++i) v[j][i] *= f.first;
+#pragma unroll
+        for (int i = 0; i < kE; ++i) v[j][i] *= f.second;
         store_run<T, kE>(p, row * p.dim + at, v[j]);
     }
 }
@@ -427,10 +439,17 @@ __global__ void __launch_bounds__(kRes > 0 ? 512 : 768) norm_stream_kernel(const
         s = reduce_row<kQuant>(s, p.group, turn);
         turn ^= 1;
         float scale = 1.0f;
-        const float f = row_factor(p, s, scale);
+        const Factors f = row_factors(p, s, scale);
         if (!live) continue;
         if (kQuant && lane == 0) p.scales[row] = scale;
-        const uint64_t f2 = pack2(f, f);
+        if (kQuant && f.first != 1.0f) {
+            const uint64_t f1 = pack2(f.first, f.first);
+#pragma unroll
+            for (int j = 0; j < kV; ++j)
+#pragma unroll
+                for (int i = 0; i < kE / 2; ++i) v[j].p[i] = mul2(v[j].p[i], f1);
+        }
+        const uint64_t f2 = pack2(f.second, f.second);
 #pragma unroll
         for (int j = 0; j < kV; ++j) {
             if (j >= runs) break;
@@ -518,15 +537,18 @@ __global__ void __launch_bounds__(512) norm_narrow_kernel(const NormParams p) {
         s = p.scales ? reduce_row<true>(s, p.group, turn) : reduce_row<false>(s, p.group, turn);
         turn ^= 1;
         float scale = 1.0f;
-        const float f = row_factor(p, s, scale);
+        const Factors f = row_factors(p, s, scale);
         if (!live) continue;
         if (p.scales && lane == 0) p.scales[row] = scale;
 #pragma unroll
         for (int j = 0; j < kV; ++j) {
             const int at = (lane + j * p.group) * kE;
             if (at >= p.dim) continue;
+            if (f.first != 1.0f)
 #pragma unroll
-            for (int i = 0; i < kE; ++i) v[j][i] *= f;
+                for (int i = 0; i < kE; ++i) v[j][i] *= f.first;
+#pragma unroll
+            for (int i = 0; i < kE; ++i) v[j][i] *= f.second;
             store_run<T, kE>(p, row * p.dim + at, v[j]);
         }
     }
@@ -709,9 +731,14 @@ __global__ void __launch_bounds__(512) norm_shifted_kernel(const NormParams p) {
         s = p.scales ? reduce_row<true>(s, p.group, turn) : reduce_row<false>(s, p.group, turn);
         turn ^= 1;
         float scale = 1.0f;
-        const float f = row_factor(p, s, scale);
+        const Factors f = row_factors(p, s, scale);
         if (!live) continue;
         if (p.scales && lane == 0) p.scales[row] = scale;
+        if (f.first != 1.0f)
+#pragma unroll
+            for (int j = 0; j < kV; ++j)
+#pragma unroll
+                for (int i = 0; i < kE; ++i) v[j][i] *= f.first;
 #pragma unroll
         for (int j = 0; j < kV; ++j) {
             const int at = (lane + j * p.group) * kE - shift;
@@ -720,12 +747,12 @@ __global__ void __launch_bounds__(512) norm_shifted_kernel(const NormParams p) {
             if (p.scales) {
                 uint16_t pairs[kE / 2];
 #pragma unroll
-                for (int i = 0; i < kE / 2; ++i) pairs[i] = e4m3x2(v[j][2 * i] * f, v[j][2 * i + 1] * f);
+                for (int i = 0; i < kE / 2; ++i) pairs[i] = e4m3x2(v[j][2 * i] * f.second, v[j][2 * i + 1] * f.second);
                 store_part(reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(p.out) + start + shift + at), pairs, lo, hi);
             } else {
                 decltype(pair_of<T>(0.0f, 0.0f)) pairs[kE / 2];
 #pragma unroll
-                for (int i = 0; i < kE / 2; ++i) pairs[i] = pair_of<T>(v[j][2 * i] * f, v[j][2 * i + 1] * f);
+                for (int i = 0; i < kE / 2; ++i) pairs[i] = pair_of<T>(v[j][2 * i] * f.second, v[j][2 * i + 1] * f.second);
                 store_part(reinterpret_cast<decltype(&pairs[0])>(static_cast<T*>(p.out) + start + shift + at), pairs, lo, hi);
             }
         }
@@ -764,10 +791,10 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const NormParams p) {
     }
     s = reduce_row<true>(s, p.group);
     float scale = 1.0f;
-    const float f = row_factor(p, s, scale);
+    const Factors f = row_factors(p, s, scale);
     if (p.scales && threadIdx.x == 0) p.scales[row] = scale;
     for (int at = threadIdx.x; at < p.dim; at += blockDim.x) {
-        const float y[1] = {value(at) * weight(at) * f};
+        const float y[1] = {value(at) * weight(at) * f.first * f.second};
         store_run<T, 1>(p, row * p.dim + at, y);
     }
 }

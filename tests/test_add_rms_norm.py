@@ -380,3 +380,35 @@ def test_packed_rows_of_uneven_width_write_nothing_else():
                     _close(buf[32:32 + n].view(rows, dim), y64, torch.bfloat16)
                 for t in (buf.float(), total):
                     assert (t[:32] == 7).all() and (t[32 + n:] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,dim,apart", [(9, 128, 0), (9, 5120, 0), (70003, 128, 0), (2503, 5120, 0), (600, 1004, 4), (600, 1001, 3),
+                                            (600, 1001, 0), (9, 6143, 0), (5, 70001, 0)])
+def test_quantised_rows_of_tiny_values(rows, dim, apart, dtype):
+    """Rows whose 448 / max|v w| is infinite in fp32 although 1 / sqrt(mean + eps) and 1 / scale are finite: their values keep
+    their size, their zeros stay zero, and the rows beside them do not change.  Few rows and many, packed, apart, uneven,
+    long.  (What an fp16 row holds is at least 6e-8, so there the weight makes the products tiny, by a power of two.)"""
+    from mindiesd import add_rms_norm_quant
+    x = torch.zeros(rows, dim + apart, dtype=dtype, device="cuda")[:, :dim].copy_(_randn(dim, rows, dim, dtype=dtype))
+    plain = add_rms_norm_quant(x)
+    tops = [1.5e-36, 1.2e-36, 1e-37, 3e-38, 1e-39]
+    tiny = list(range(min(rows, 5))) + ([rows // 2, rows - 1] if rows > 10 else [])
+    factor = 1.0 if dtype != torch.float16 else 2.0 ** -110
+    for i, row in enumerate(tiny):
+        x[row] *= tops[i % 5] / factor / x[row].abs().max().float()
+        x[row, ::3] = 0
+        x[row, 1] = tops[i % 5] / factor
+    weight = None if dtype != torch.float16 else torch.full((dim,), factor, device="cuda")
+    q, s = add_rms_norm_quant(x, weight)
+    y64, _ = ob.rms_norm(x[tiny], weight)
+    assert torch.isfinite(s).all() and not q.float().isnan().any()
+    assert torch.count_nonzero(q[tiny][:, ::3].float()) == 0
+    _close_quant(q[tiny], s[tiny], y64)
+    if weight is None:
+        keep = torch.ones(rows, dtype=torch.bool, device="cuda")
+        keep[tiny] = False
+        assert torch.equal(q[keep].float(), plain[0][keep].float()) and torch.equal(s[keep], plain[1][keep])
+    else:
+        _close_quant(q, s, ob.rms_norm(x, weight)[0])
