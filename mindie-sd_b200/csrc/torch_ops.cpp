@@ -830,15 +830,26 @@ at::Tensor as_rows(const at::Tensor& x, int64_t* rows, int64_t* stride) {
     return x;
 }
 
-bool records_gradients(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+// Whether a derivative is expected of what is computed from t, backward or forward.
+bool wants_derivative(const at::Tensor& t) {
+    return (at::GradMode::is_enabled() && t.requires_grad()) ||
+           (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined());
+}
 
 using MaybeTensor = c10::optional<at::Tensor>;
+
+bool wants_derivative(const MaybeTensor& t) { return t.has_value() && t->defined() && wants_derivative(*t); }
+
+// The operators without derivatives refuse inputs of which one is expected where autograd stands: the tensors of a
+// functional transform (torch.func.jvp, torch.func.grad) arrive at the implementation unwrapped, and would come back
+// without it.
+constexpr const char* kNoDerivative = "mindiesd: no derivative, but an input requires a gradient or carries a tangent";
 
 std::tuple<at::Tensor, MaybeTensor, MaybeTensor> add_rms_norm_cuda(const at::Tensor& x, const MaybeTensor& weight,
                                                                    const MaybeTensor& residual, double eps, bool quant,
                                                                    bool quant_only) {
     const at::ScalarType type = x.scalar_type();
-    TORCH_CHECK(x.is_cuda() && x.dim() >= 1 && x.size(-1) > 0 && !records_gradients(x), "add_rms_norm: x must be a CUDA tensor [..., D]");
+    TORCH_CHECK(x.is_cuda() && x.dim() >= 1 && x.size(-1) > 0, "add_rms_norm: x must be a CUDA tensor [..., D]");
     TORCH_CHECK(type == at::kBFloat16 || type == at::kHalf || type == at::kFloat, "add_rms_norm: x must be bf16, fp16 or fp32");
     TORCH_CHECK(eps > 1e-38 && eps < 1e30, "add_rms_norm: eps must be positive and normal in fp32");
     const int64_t d = x.size(-1);
@@ -852,7 +863,7 @@ std::tuple<at::Tensor, MaybeTensor, MaybeTensor> add_rms_norm_cuda(const at::Ten
     if (weight.has_value()) {
         const at::Tensor& w = weight.value();
         TORCH_CHECK(w.is_cuda() && w.device() == x.device() && w.dim() == 1 && w.size(0) == d &&
-                        (w.scalar_type() == type || w.scalar_type() == at::kFloat) && !records_gradients(w),
+                        (w.scalar_type() == type || w.scalar_type() == at::kFloat),
                     "add_rms_norm: weight must be [D] on the device of x, in its type or fp32");
         wr = w.contiguous();
         a.weight = wr.data_ptr();
@@ -861,7 +872,7 @@ std::tuple<at::Tensor, MaybeTensor, MaybeTensor> add_rms_norm_cuda(const at::Ten
     if (residual.has_value()) {
         const at::Tensor& r = residual.value();
         TORCH_CHECK(r.is_cuda() && r.device() == x.device() && r.sizes() == x.sizes() &&
-                        (r.scalar_type() == type || r.scalar_type() == at::kFloat) && !records_gradients(r),
+                        (r.scalar_type() == type || r.scalar_type() == at::kFloat),
                     "add_rms_norm: residual must have the shape and the device of x, in its type or fp32");
         int64_t rows = 0;
         rr = as_rows(r, &rows, &a.residual_stride);
@@ -886,6 +897,15 @@ std::tuple<at::Tensor, MaybeTensor, MaybeTensor> add_rms_norm_cuda(const at::Ten
     c10::cuda::CUDAGuard guard(x.device());
     check_rc(mindiesd_add_rms_norm(&a, stream_of(x)), "mindiesd_add_rms_norm");
     return {out, made(scales), made(residual_out)};
+}
+
+using NormFn = std::tuple<at::Tensor, MaybeTensor, MaybeTensor>(const at::Tensor&, const MaybeTensor&, const MaybeTensor&, double, bool, bool);
+std::tuple<at::Tensor, MaybeTensor, MaybeTensor> add_rms_norm_autograd(c10::DispatchKeySet keys, const at::Tensor& x,
+                                                                       const MaybeTensor& weight, const MaybeTensor& residual,
+                                                                       double eps, bool quant, bool quant_only) {
+    TORCH_CHECK(!wants_derivative(x) && !wants_derivative(weight) && !wants_derivative(residual), kNoDerivative);
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("mindiesd::add_rms_norm", "").typed<NormFn>();
+    return op.redispatch(keys & c10::after_autograd_keyset, x, weight, residual, eps, quant, quant_only);
 }
 
 // ---- matrix product with bias, activation, gate and residual ------------------------------------------------
@@ -961,7 +981,7 @@ at::Tensor linear_fwd_cuda(const at::Tensor& x, const at::Tensor& weight, const 
     const at::ScalarType type = x.scalar_type();
     const bool fp8 = type == at::kFloat8_e4m3fn;
     TORCH_CHECK(fp8 || type == at::kBFloat16 || type == at::kHalf, "linear_fwd: x must be bf16, fp16 or e4m3");
-    auto usable = [&](const at::Tensor& t) { return t.is_cuda() && t.device() == x.device() && !records_gradients(t); };
+    auto usable = [&](const at::Tensor& t) { return t.is_cuda() && t.device() == x.device(); };
     auto is_float = [](const at::Tensor& t) {
         return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf || t.scalar_type() == at::kFloat;
     };
@@ -1043,6 +1063,20 @@ at::Tensor linear_fwd_cuda(const at::Tensor& x, const at::Tensor& weight, const 
     a.activation = act;
     check_rc(mindiesd_linear_fwd(&a, stream_of(x)), "mindiesd_linear_fwd");
     return out;
+}
+
+using LinearFn = at::Tensor(const at::Tensor&, const at::Tensor&, const MaybeTensor&, const MaybeTensor&, const MaybeTensor&,
+                            const MaybeTensor&, const MaybeTensor&, c10::string_view, c10::optional<at::ScalarType>);
+at::Tensor linear_fwd_autograd(c10::DispatchKeySet keys, const at::Tensor& x, const at::Tensor& weight, const MaybeTensor& bias,
+                               const MaybeTensor& residual, const MaybeTensor& gate, const MaybeTensor& x_scale,
+                               const MaybeTensor& weight_scale, c10::string_view activation,
+                               c10::optional<at::ScalarType> out_dtype) {
+    TORCH_CHECK(!wants_derivative(x) && !wants_derivative(weight) && !wants_derivative(bias) && !wants_derivative(residual) &&
+                    !wants_derivative(gate) && !wants_derivative(x_scale) && !wants_derivative(weight_scale),
+                kNoDerivative);
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("mindiesd::linear_fwd", "").typed<LinearFn>();
+    return op.redispatch(keys & c10::after_autograd_keyset, x, weight, bias, residual, gate, x_scale, weight_scale, activation,
+                         out_dtype);
 }
 
 }  // namespace
@@ -1129,4 +1163,9 @@ TORCH_LIBRARY_IMPL(mindiesd, CUDA, m) {
     m.impl("fp8_attention", &fp8_attention_cuda);
     m.impl("add_rms_norm", &add_rms_norm_cuda);
     m.impl("linear_fwd", &linear_fwd_cuda);
+}
+
+TORCH_LIBRARY_IMPL(mindiesd, Autograd, m) {
+    m.impl("add_rms_norm", &add_rms_norm_autograd);
+    m.impl("linear_fwd", &linear_fwd_autograd);
 }

@@ -4,8 +4,8 @@ addition.  Operands are bf16 or fp16, or e4m3 with their scales (`token_quant_pr
 `add_rms_norm_quant`); the reference leaves the first to torch.nn.Linear and the second to the quantised
 layers of mindiesd/quantization/layer.py of MindIE-SD.
 
-Inference only: there is no backward pass, so tensors that require gradients are refused while
-gradients are recorded.
+Inference only: there is no backward pass and no forward-mode derivative, so tensors that require gradients are
+refused while gradients are recorded, and so are tensors that carry a tangent.
 """
 import torch
 

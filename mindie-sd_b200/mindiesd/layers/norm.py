@@ -3,10 +3,11 @@ root-mean-square norm in one pass; `RMSNorm` of mindiesd/layers/norm.py of MindI
 that precedes it) and `add_rms_norm_quant`, whose output is e4m3 with one scale per token, ready for
 `linear_forward`.
 
-Inference only: there is no backward pass, so tensors that require gradients are refused while
-gradients are recorded.
+Inference only: there is no backward pass and no forward-mode derivative, so tensors that require gradients are
+refused while gradients are recorded, and so are tensors that carry a tangent.
 """
 import torch
+from torch.autograd import forward_ad
 
 from . import _custom_ops  # noqa: F401  (registers the fake implementations)
 from ..utils.exception import ParametersInvalid
@@ -16,11 +17,11 @@ _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def refuse_gradients(where, *tensors):
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise ParametersInvalid(f"{where} has no backward pass; call it under torch.no_grad() or "
-                                        "torch.inference_mode().")
+    given = [t for t in tensors if t is not None]
+    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
+        raise ParametersInvalid(f"{where} has no backward pass; call it under torch.no_grad() or torch.inference_mode().")
+    if torch._C._is_fwd_grad_enabled() and any(forward_ad.unpack_dual(t).tangent is not None for t in given):
+        raise ParametersInvalid(f"{where} has no forward-mode derivative, but an input carries a tangent.")
 
 
 def _explain(where, x, weight, residual, eps):
