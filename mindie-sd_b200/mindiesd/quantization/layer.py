@@ -68,7 +68,9 @@ class FP8DynamicLinear(nn.Module):
 
     forward(x, activation=, residual=, gate=, out_dtype=): x is a bf16 / fp16 / fp32 tensor [..., K], or the pair
     (e4m3 [..., K], scales [..., 1]) that add_rms_norm_quant returns; the other arguments are linear_forward's.
-    The output has the type of x (bfloat16 for fp32 and for a pair) unless out_dtype or a residual says otherwise."""
+    The output has the type of x (bfloat16 for fp32 and for a pair) unless out_dtype or a residual says otherwise.
+
+    Converting the module to another dtype converts the bias alone."""
 
     def __init__(self, prefix=None, weights=None):
         super().__init__()
@@ -96,6 +98,14 @@ class FP8DynamicLinear(nn.Module):
         if linear.bias is not None:
             weights["linear.bias"] = linear.bias
         return cls("linear", weights)
+
+    def _apply(self, fn, recurse=True):
+        # What is stored is the e4m3 values and their fp32 scales: module.to(dtype), .half() and the like, which convert
+        # every floating-point buffer, leave these two as they are; a move to another device takes them along.
+        def same_type(t):
+            moved = fn(t)
+            return moved if moved.dtype == t.dtype else t.to(moved.device)
+        return super()._apply(lambda t: same_type(t) if t is self.weight or t is self.weight_scale else fn(t), recurse)
 
     def forward(self, x, activation="none", residual=None, gate=None, out_dtype=None):
         if isinstance(x, tuple):

@@ -178,3 +178,38 @@ def test_calls_back_to_back():
             got.zero_()
             graph.replay()
             assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("convert,bias_dtype", [(lambda m: m.to(torch.bfloat16), torch.bfloat16), (lambda m: m.half(), torch.float16),
+                                                (lambda m: m.float(), torch.float32), (lambda m: m.to("cpu", torch.float16), torch.float16),
+                                                (lambda m: m.type(torch.bfloat16), torch.bfloat16), (lambda m: m.half().bfloat16(), torch.bfloat16)])
+def test_dtype_conversions_leave_the_stored_weights(convert, bias_dtype):
+    """Of a module that holds the layer, and of the layer itself: the e4m3 values and their scales keep type and bits."""
+    from mindiesd import FP8DynamicLinear
+    g = torch.Generator().manual_seed(1)
+    weight = torch.randn(8, 16, generator=g).to(torch.float8_e4m3fn)
+    scale, bias = torch.rand(8, generator=g), torch.randn(8, generator=g)
+    for wrap in (lambda layer: layer, lambda layer: torch.nn.Sequential(torch.nn.Linear(16, 16), layer)):
+        layer = FP8DynamicLinear("p", {"p.weight": weight, "p.weight_scale": scale, "p.bias": bias})
+        convert(wrap(layer))
+        assert layer.weight.dtype == torch.float8_e4m3fn and torch.equal(layer.weight.float(), weight.float())
+        assert layer.weight_scale.dtype == torch.float32 and torch.equal(layer.weight_scale, scale)
+        assert layer.bias.dtype == bias_dtype
+    layer.to("meta")
+    assert layer.weight.is_meta and layer.weight_scale.is_meta and layer.weight.dtype == torch.float8_e4m3fn
+    assert layer(torch.zeros(3, 16, dtype=bias_dtype, device="meta")).shape == (3, 8)
+    layer.to_empty(device="cpu")
+    assert layer.weight.device.type == "cpu" and layer.weight.dtype == torch.float8_e4m3fn and layer.weight_scale.dtype == torch.float32
+
+
+@pytest.mark.gpu
+def test_converted_layer_runs():
+    from mindiesd import FP8DynamicLinear
+    linear = torch.nn.Linear(384, 264, device="cuda", dtype=torch.bfloat16)
+    layer = FP8DynamicLinear.from_linear(linear)
+    x = tn._randn(1, 5, 384, dtype=torch.bfloat16)
+    want = layer(x)
+    for convert in (lambda m: m.to(torch.float32), lambda m: m.to(torch.bfloat16), lambda m: m.cpu().bfloat16().cuda()):
+        convert(torch.nn.Sequential(layer))
+        assert layer.weight.is_cuda and layer.weight_scale.is_cuda
+        assert torch.equal(layer(x), want)
