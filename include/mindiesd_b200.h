@@ -481,7 +481,7 @@ int mindiesd_add_rms_norm(const mindiesd_norm_args* args, void* stream);
  * weight_stride elements apart (multiples of 16 bytes, 16-byte aligned; k itself may be any).  Products are
  * accumulated in fp32, the epilogue runs in fp32, one rounding to out_dtype (bf16 or fp16).
  * x_scale, weight_scale: e4m3 operands only (required then): fp32 [m] and [n], or one value each
- * (x_scale_single / weight_scale_single).
+ * (x_scale_single / weight_scale_single); the accumulated sum takes the one, then the other.
  * Each optional (NULL): bias [n]; residual [m, n] in out_dtype; gate [ceil(m / rows_per_gate), n], row i using
  * gate row i / rows_per_gate (one gate per sample of a batch).  bias and gate are bf16, fp16 or fp32, each
  * on its own.  out: rows out_stride elements apart; must not overlap an input.

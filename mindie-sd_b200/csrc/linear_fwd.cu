@@ -561,12 +561,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
             // Values of a unit's columns in this lane's row (the j-th unit of the warp), from accumulator to output.
             auto finish = [&](uint64_t (&v)[kUnit / 2], const uint32_t (&old)[kUnit / 2], int j, int col0) {
                 const ulonglong2* at = reinterpret_cast<const ulonglong2*>(cols + j * kUnit);  // two pairs of columns per load
-                if constexpr (kFp8) {
+                if constexpr (kFp8) {  // one scale after the other: their product alone may be out of range
 #pragma unroll
                     for (int i = 0; i < kUnit / 4; ++i) {
                         const ulonglong2 f = at[kCols / 4 + i];
-                        v[2 * i] = mul2(v[2 * i], mul2(f.x, both(xs)));
-                        v[2 * i + 1] = mul2(v[2 * i + 1], mul2(f.y, both(xs)));
+                        v[2 * i] = mul2(mul2(v[2 * i], both(xs)), f.x);
+                        v[2 * i + 1] = mul2(mul2(v[2 * i + 1], both(xs)), f.y);
                     }
                 }
                 if (e.bias) {
@@ -734,7 +734,7 @@ __global__ void __launch_bounds__(kSwapThreads) linear_swap_kernel(const __grid_
         if (kFp8) {
             const float xs = __ldg(e.x_scale + row * e.x_scale_step);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] *= xs * scale[i];
+            for (int i = 0; i < 4; ++i) v[i] = v[i] * xs * scale[i];
         }
         uint64_t pairs[2] = {pack2(v[0] + b[0], v[1] + b[1]), pack2(v[2] + b[2], v[3] + b[3])};
         activate(pairs, e.act);

@@ -537,3 +537,23 @@ def test_activations_over_their_range(act, m):
     y = linear_forward(x, eye, bias, activation=act)
     assert (y[:, 1] == float("inf")).all() and y[:, 2].isnan().all()
     assert (y[:, 5].float().abs() < 1e-15).all() and (y[:, [0, 3, 4, 6]] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", [(5, 1024, 40), (100, 520, 131), (4400, 64, 264), (4400, 320, 257)])
+def test_scales_whose_product_is_out_of_range(m, k, n):
+    """A row scale and a column scale are finite each, but their product may be subnormal or infinite in fp32 where the result
+    is neither: rows of the quantiser's smallest scale, and zeros under two large ones."""
+    from mindiesd import linear_forward
+    g = torch.Generator(device="cuda").manual_seed(m)
+    x, w = ((200 + 248 * torch.rand(rows, k, generator=g, device="cuda")).to(torch.float8_e4m3fn) for rows in (m, n))
+    xs = (1 + torch.rand(m, 1, generator=g, device="cuda")) * 2.0 ** -126
+    ws = (1 + torch.rand(n, generator=g, device="cuda")) * 2.0 ** -18
+    kw = dict(x_scale=xs, weight_scale=ws)
+    got = linear_forward(x, w, **kw)
+    _check(got, x, w, torch.bfloat16, k, **kw)
+    x[3], xs[3], ws[7] = 0, 2.0 ** 100, 2.0 ** 100
+    got = linear_forward(x, w, **kw)
+    assert (got[3] == 0).all()
+    keep = [i for i in range(m) if i != 3]
+    _check(got[keep], x[keep], w, torch.bfloat16, k, x_scale=xs[keep], weight_scale=ws)
