@@ -445,8 +445,8 @@ int mindiesd_rope(const mindiesd_rope_args* args, void* stream);
  *   residual_out = v rounded once to the residual's type; required exactly when residual is given
  * The squares are summed in fp32: a row with values beyond 1.8e19 overflows the sum and comes out as zeros.
  * x, residual: rows x_stride / residual_stride elements apart, channels contiguous; weight (NULL = ones):
- * [dim]; out and residual_out: contiguous [rows, dim], not overlapping an input (refused).  Any dim and any alignment of the element's size;
- * 16-byte aligned rows are fastest.  residual and weight are in the type of x or fp32, each on its own.
+ * [dim]; out and residual_out: contiguous [rows, dim].  No output may overlap an input or another output (refused).
+ * Any dim and any alignment of the element's size; 16-byte aligned rows are fastest.  residual and weight are in the type of x or fp32, each on its own.
  * quant_only != 0: y = x (no norm; weight and residual must be NULL, out_dtype MINDIESD_E4M3; with an
  * infinity in a row its scale is infinity).
  *

@@ -1003,16 +1003,26 @@ extern "C" int mindiesd_add_rms_norm(const mindiesd_norm_args* a, void* stream_)
     if (a->weight && !aligned(a->weight, dtype_bytes(a->weight_dtype))) return MINDIESD_E_STRIDE;
     if (!a->quant_only && !(a->eps > 0.0f && a->eps < 1e30f)) return MINDIESD_E_VALUE;
     if (a->quant_only && (a->weight || a->residual || a->out_dtype != MINDIESD_E4M3)) return MINDIESD_E_VALUE;
-    // Rows are fetched ahead, and long ones read twice, so nothing may be written where an input is still read.
-    const int64_t count = a->rows * a->dim;
-    auto overlap = [&](const void* out, int out_bytes, const void* in, int64_t stride, int in_bytes) {
-        const uintptr_t o = reinterpret_cast<uintptr_t>(out), i = reinterpret_cast<uintptr_t>(in);
-        return out && in && o < i + static_cast<uintptr_t>((a->rows - 1) * stride + a->dim) * in_bytes && i < o + static_cast<uintptr_t>(count) * out_bytes;
+    // Rows are fetched ahead, and long ones read twice, so nothing may be written where an input is still read, nor where
+    // another output is written.
+    struct Span {
+        uintptr_t first, end;
+        bool written;
+    };
+    auto span = [](const void* at, int64_t rows, int64_t stride, int64_t width, int bytes, bool written) {
+        const uintptr_t first = reinterpret_cast<uintptr_t>(at);
+        return Span{first, at ? first + static_cast<uintptr_t>((rows - 1) * stride + width) * bytes : first, written};
     };
     const int oe = dtype_bytes(a->out_dtype), re = a->residual ? dtype_bytes(a->residual_dtype) : 0;
-    if (overlap(a->out, oe, a->x, a->x_stride, e) || overlap(a->out, oe, a->residual, a->residual_stride, re) ||
-        overlap(a->residual_out, re, a->x, a->x_stride, e) || overlap(a->residual_out, re, a->residual, a->residual_stride, re))
-        return MINDIESD_E_VALUE;
+    const Span spans[] = {span(a->x, a->rows, a->x_stride, a->dim, e, false),
+                          span(a->residual, a->rows, a->residual_stride, a->dim, re, false),
+                          span(a->weight, 1, 0, a->dim, a->weight ? dtype_bytes(a->weight_dtype) : 0, false),
+                          span(a->out, a->rows, a->dim, a->dim, oe, true),
+                          span(a->residual_out, a->rows, a->dim, a->dim, re, true),
+                          span(a->out_dtype == MINDIESD_E4M3 ? a->scales : nullptr, a->rows, 1, 1, 4, true)};
+    for (const Span& s : spans)
+        for (const Span& t : spans)
+            if (&s != &t && s.written && s.first < t.end && t.first < s.end) return MINDIESD_E_VALUE;
     NormParams p = {};
     p.x = a->x;
     p.residual = a->residual;

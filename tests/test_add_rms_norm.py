@@ -412,3 +412,52 @@ def test_quantised_rows_of_tiny_values(rows, dim, apart, dtype):
         assert torch.equal(q[keep].float(), plain[0][keep].float()) and torch.equal(s[keep], plain[1][keep])
     else:
         _close_quant(q, s, ob.rms_norm(x, weight)[0])
+
+
+@pytest.mark.parametrize("written,other,bytes_of_other", [("out", "weight", 128), ("residual_out", "weight", 128), ("scales", "x", 608), ("scales", "residual", 608),
+                                                          ("scales", "weight", 128), ("scales", "out", 256), ("scales", "residual_out", 512), ("out", "residual_out", 512)])
+def test_outputs_over_weights_and_each_other_are_refused(written, other, bytes_of_other):
+    """Addresses that overlap by one element; refused before anything reads them, so no device is needed."""
+    from mindiesd import _cabi
+
+    def code(**where):
+        a = _cabi.NormArgs()
+        a.rows, a.dim, a.eps = 4, 64, 1e-6
+        a.dtype = a.residual_dtype = a.weight_dtype = _cabi.BF16
+        a.out_dtype = _cabi.E4M3
+        a.x, a.residual, a.weight, a.out, a.residual_out = 1 << 20, 2 << 20, 5 << 20, 3 << 20, 4 << 20
+        a.scales = 6 << 20
+        a.x_stride = a.residual_stride = 80
+        for name, at in where.items():
+            setattr(a, name, at)
+        return _cabi.lib().mindiesd_add_rms_norm(ctypes.byref(a), None)
+    place = {"x": 1 << 20, "residual": 2 << 20, "weight": 5 << 20, "out": 3 << 20, "residual_out": 4 << 20}[other]
+    size = {"out": 256, "residual_out": 512, "scales": 16}[written]
+    for delta in (0, bytes_of_other - 4, -(size - 4)):
+        assert code(**{written: place + delta}) == -5
+
+
+@pytest.mark.gpu
+def test_operands_side_by_side_are_taken():
+    """Inputs and outputs that follow one another in one buffer without a gap."""
+    from mindiesd import _cabi
+    rows, dim = 4, 64
+    x, w = _randn(31, rows, dim, dtype=torch.bfloat16), _randn(32, dim, dtype=torch.bfloat16)
+    sizes = {"x": 512, "out": 256, "residual": 512, "residual_out": 512, "weight": 128, "scales": 16}
+    for order in (list(sizes), list(sizes)[::-1]):
+        buf, at = torch.zeros(sum(sizes.values()), dtype=torch.uint8, device="cuda"), {}
+        for name in order:
+            at[name] = buf[sum(t.numel() for t in at.values()):][:sizes[name]]
+        for name, t in (("x", x), ("residual", x), ("weight", w)):
+            at[name].copy_(t.view(torch.uint8).flatten())
+        a = _cabi.NormArgs()
+        for name, t in at.items():
+            setattr(a, name, t.data_ptr())
+        a.rows, a.dim, a.x_stride, a.residual_stride, a.eps = rows, dim, dim, dim, 1e-6
+        a.dtype = a.residual_dtype = a.weight_dtype = _cabi.BF16
+        a.out_dtype = _cabi.E4M3
+        _cabi.check(_cabi.lib().mindiesd_add_rms_norm(ctypes.byref(a), _cabi.current_stream_ptr(x.device)), "mindiesd_add_rms_norm")
+        y64, v64 = ob.rms_norm(x, w, x)
+        _close(at["residual_out"].view(torch.bfloat16).view(rows, dim), v64, torch.bfloat16)
+        _close_quant(at["out"].view(torch.float8_e4m3fn).view(rows, dim), at["scales"].view(torch.float32)[:, None], y64)
+        assert torch.equal(at["x"], x.view(torch.uint8).flatten()) and torch.equal(at["weight"], w.view(torch.uint8).flatten())
