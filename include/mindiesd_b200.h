@@ -443,7 +443,8 @@ int mindiesd_rope(const mindiesd_rope_args* args, void* stream);
  *   scales       fp32 [rows], e4m3 only: max|y| / 448 of the row (at least 2^-126), 1 for a row of zeros;
  *                real value = stored value * scale.  A NaN or infinity in a row makes its scale NaN
  *   residual_out = v rounded once to the residual's type; required exactly when residual is given
- * The squares are summed in fp32: a row with values beyond 1.8e19 overflows the sum and comes out as zeros.
+ * The squares are summed in fp32: a row whose sum of squares passes 3.4e38 (a root mean square of 1.8e19 / sqrt(dim): 2.6e17
+ * for 5120 channels) overflows it and comes out as zeros, with a scale of 1.
  * x, residual: rows x_stride / residual_stride elements apart, channels contiguous; weight (NULL = ones):
  * [dim]; out and residual_out: contiguous [rows, dim].  No output may overlap an input or another output (refused).
  * Any dim and any alignment of the element's size; 16-byte aligned rows are fastest.  residual and weight are in the type of x or fp32, each on its own.

@@ -74,7 +74,8 @@ def add_rms_norm(x, weight=None, residual=None, eps=1e-6):
     without a residual) and one rounding to the type of x.  x: [..., D] bf16, fp16 or fp32; weight [D] (None:
     ones) and residual [..., D] in the type of x or fp32.  Returns y, or (y, v rounded to the residual's type)
     when a residual is given.  Leading dimensions that share one row stride (slices of a packed projection)
-    are read in place.  The squares are summed in fp32: values beyond 1.8e19 overflow it and give a row of zeros."""
+    are read in place.  The squares are summed in fp32: a row whose sum passes 3.4e38 (a root mean square of 1.8e19 /
+    sqrt(D), 2.6e17 for 5120 channels) gives zeros."""
     y, _, total = _run("add_rms_norm", x, weight, residual, eps, False)
     return y if residual is None else (y, total)
 
@@ -82,6 +83,7 @@ def add_rms_norm(x, weight=None, residual=None, eps=1e-6):
 def add_rms_norm_quant(x, weight=None, residual=None, eps=1e-6):
     """The same norm with its output in e4m3 and one scale per token, taken on the fp32 values: returns
     (e4m3 [..., D], fp32 scales [..., 1]), with the residual's sum as a third where one is given; real value =
-    stored * scale, scale = max|y| / 448 (1 for a token of zeros, NaN for one that holds a NaN or an infinity)."""
+    stored * scale, scale = max|y| / 448 (1 for a token of zeros, or one whose sum of squares overflows as there; NaN for
+    one that holds a NaN or an infinity)."""
     q, scale, total = _run("add_rms_norm_quant", x, weight, residual, eps, True)
     return (q, scale) if residual is None else (q, scale, total)

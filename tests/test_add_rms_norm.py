@@ -461,3 +461,21 @@ def test_operands_side_by_side_are_taken():
         _close(at["residual_out"].view(torch.bfloat16).view(rows, dim), v64, torch.bfloat16)
         _close_quant(at["out"].view(torch.float8_e4m3fn).view(rows, dim), at["scales"].view(torch.float32)[:, None], y64)
         assert torch.equal(at["x"], x.view(torch.uint8).flatten()) and torch.equal(at["weight"], w.view(torch.uint8).flatten())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,dim,apart", [(4, 1, 0), (4, 128, 0), (9, 5120, 0), (2503, 5120, 0), (600, 1001, 3), (600, 1001, 0), (4, 70001, 0)])
+def test_rows_around_the_largest_sum_of_squares(rows, dim, apart):
+    """A root mean square of 0.9 and of 1.1 times sqrt(largest fp32 / dim): the values, and zeros with a scale of 1."""
+    from mindiesd import add_rms_norm, add_rms_norm_quant
+    bound = (torch.finfo(torch.float32).max / dim) ** 0.5
+    x = torch.empty(rows, dim + apart, device="cuda")[:, :dim]
+    sign = torch.randint(0, 2, (rows, dim), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda") * 2.0 - 1
+    x.copy_(sign * 0.9 * bound)
+    x[rows // 2] *= 1.1 / 0.9
+    keep = torch.arange(rows, device="cuda") != rows // 2
+    y64 = ob.rms_norm(x)[0]
+    y, (q, s) = add_rms_norm(x), add_rms_norm_quant(x)
+    _close(y[keep], y64[keep], torch.float32)
+    _close_quant(q[keep], s[keep], y64[keep])
+    assert (y[~keep] == 0).all() and (q[~keep].float() == 0).all() and (s[~keep] == 1).all()
