@@ -891,6 +891,8 @@ cudaError_t launch_shifted(const NormParams& p, int threads, int smem, cudaStrea
 constexpr int kShiftedMost = 3;         // runs of a thread
 constexpr int kShiftedMaxDim = 11000;   // the weights in 48 KB of shared memory
 
+constexpr int kHalfRunsMaxDim = 512 * 16;  // 16 elements per thread of the largest block of norm_narrow_kernel
+
 template <typename T>
 cudaError_t launch_shifted(NormParams p, cudaStream_t stream) {
     constexpr int kE = 16 / sizeof(T);
@@ -967,9 +969,10 @@ cudaError_t launch_typed(const NormParams& p, cudaStream_t stream) {
                         starts(p.residual, 16) && starts(p.residual_out, 16) && starts(p.out, p.scales ? kWide : 16);
     // Runs of half the width suit rows that they divide, as long as no residual adds to the loads or the rows are short
     // (bf16, half / shared whole ones: 20000 x 1004 20 / 27 us, with a residual 34 / 40; 10000 x 1500 19 / 22 and 31 / 28;
-    // 6000 x 5124 42 / 44 and 66 / 53).
+    // 6000 x 5124 42 / 44 and 66 / 53), and as long as a block's registers hold the row (6000 x 8196 shared 87, and 186 by
+    // norm_long_kernel).
     if constexpr (kWide == 8) {
-        if (fits(4) && (!p.residual || p.dim <= 1024 || !packed)) return launch_rows<T, 4>(p, stream);
+        if (fits(4) && ((!p.residual && p.dim <= kHalfRunsMaxDim) || p.dim <= 1024 || !packed)) return launch_rows<T, 4>(p, stream);
     }
     if (packed && p.dim >= kWide && p.dim <= kShiftedMaxDim && p.dim <= kWide * (512 * kShiftedMost - 2)) return launch_shifted<T>(p, stream);
     return launch_rows<T, 1>(p, stream);

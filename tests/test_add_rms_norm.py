@@ -479,3 +479,18 @@ def test_rows_around_the_largest_sum_of_squares(rows, dim, apart):
     _close(y[keep], y64[keep], torch.float32)
     _close_quant(q[keep], s[keep], y64[keep])
     assert (y[~keep] == 0).all() and (q[~keep].float() == 0).all() and (s[~keep] == 1).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("dim", [8188, 8192, 8196, 10996, 11000, 11004])
+def test_packed_rows_that_four_divides(dim, dtype):
+    """On both sides of the longest row that runs of four elements keep in registers, and of the longest that shared
+    memory keeps the weights of."""
+    from mindiesd import add_rms_norm, add_rms_norm_quant
+    for rows, weight in ((3, dtype), (1301, torch.float32), (700, None)):
+        x = _randn(dim + rows, rows, dim, dtype=dtype)
+        w = None if weight is None else _randn(1, dim, dtype=weight)
+        y64 = ob.rms_norm(x, w)[0]
+        _close(add_rms_norm(x, w), y64, dtype)
+        _close_quant(*add_rms_norm_quant(x, w), y64)
