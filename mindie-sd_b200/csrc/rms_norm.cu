@@ -851,6 +851,9 @@ cudaError_t launch_stream(const NormParams& p, int threads, cudaStream_t stream)
                     : launch_stream_as<T, kE, kV, kRes, false>(p, threads, stream);
 }
 
+constexpr int kMostRuns = 6, kMostWithResidual = 3;  // of 16 bytes, by one thread of a block of up to 512 (launch_rows)
+static_assert(stream_smem<kMostRuns, 0>(512) <= kMaxSmem && stream_smem<kMostWithResidual, 32>(512) <= kMaxSmem, "shared memory of the stream kernel");
+
 // Rows of 16-byte runs.
 template <typename T, int kV>
 cudaError_t launch_wide(const NormParams& p, int threads, cudaStream_t stream) {
@@ -859,12 +862,10 @@ cudaError_t launch_wide(const NormParams& p, int threads, cudaStream_t stream) {
     // Worth its longer start only where a block walks several rows: 2000 rows of 5120 bf16 with a residual 15.6 us
     // (norm_row_kernel 17.4), 300 rows as fast either way.
     if (blocks > kStreamBlocks && threads <= 512) {
-        if (!p.residual) {
-            if (stream_smem<kV, 0>(threads) <= kMaxSmem) return launch_stream<T, kE, kV, 0>(p, threads, stream);
-        } else if (p.residual_fp32) {
-            if (stream_smem<kV, 4 * kE>(threads) <= kMaxSmem) return launch_stream<T, kE, kV, 4 * kE>(p, threads, stream);
-        } else {
-            if (stream_smem<kV, 16>(threads) <= kMaxSmem) return launch_stream<T, kE, kV, 16>(p, threads, stream);
+        if (!p.residual) return launch_stream<T, kE, kV, 0>(p, threads, stream);
+        if constexpr (kV <= kMostWithResidual) {  // more runs come with blocks of 1024 threads alone (launch_rows)
+            if (p.residual_fp32) return launch_stream<T, kE, kV, 4 * kE>(p, threads, stream);
+            return launch_stream<T, kE, kV, 16>(p, threads, stream);
         }
     }
     return launch(norm_row_kernel<T, kE, kV>, p, blocks, threads, 0, stream);
@@ -914,7 +915,7 @@ cudaError_t launch_rows(NormParams p, cudaStream_t stream) {
     // The smallest group of threads that holds the row in so many runs each: three 16-byte runs (75600 x 5120 bf16
     // with a residual 471 us, with six runs 490; 300 rows 4.5 us, six 5.7), six where the row is wide and has no
     // residual (quantised 238 us, three 311: the reduction over twice the warps costs more than the loads).
-    const int most = !kWide ? 16 / kE : p.residual || runs <= 384 ? 3 : 6;
+    const int most = !kWide ? 16 / kE : p.residual || runs <= 384 ? kMostWithResidual : kMostRuns;
     int group = 1;
     while (group < 512 && group * most < runs) group *= 2;
     int per_thread = (runs + group - 1) / group;
@@ -922,7 +923,7 @@ cudaError_t launch_rows(NormParams p, cudaStream_t stream) {
         group = 1024;
         per_thread = (runs + group - 1) / group;
     }
-    if (per_thread > (kWide ? 6 : most)) {
+    if (per_thread > (kWide ? kMostRuns : most)) {
         p.group = 1024;
         return launch(norm_long_kernel<T>, p, p.rows, 1024, 0, stream);
     }
