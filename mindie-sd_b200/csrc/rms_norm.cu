@@ -913,9 +913,11 @@ cudaError_t launch_rows(NormParams p, cudaStream_t stream) {
     const int runs = (p.dim + kE - 1) / kE;
     constexpr bool kWide = kE * sizeof(T) == 16;
     // The smallest group of threads that holds the row in so many runs each: three 16-byte runs (75600 x 5120 bf16
-    // with a residual 471 us, with six runs 490; 300 rows 4.5 us, six 5.7), six where the row is wide and has no
-    // residual (quantised 238 us, three 311: the reduction over twice the warps costs more than the loads).
-    const int most = !kWide ? 16 / kE : p.residual || runs <= 384 ? kMostWithResidual : kMostRuns;
+    // with a residual 471 us, with six runs 490), six where the rows are wide, have no residual and are many enough for
+    // norm_stream_kernel (quantised 238 us, three 311: the reduction over twice the warps costs more than the loads).
+    // Fewer rows of that kind take three: bf16 300 x 5120 3.5 us, six 5.2; 590 x 6144 4.0 and 9.4 (registers of
+    // norm_row_kernel spill); from 592 rows on it is about even (1000 x 5120 5.5 and 5.6, quantised 5.9 and 5.7).
+    const int most = !kWide ? 16 / kE : p.residual || runs <= 384 || p.rows <= kStreamBlocks ? kMostWithResidual : kMostRuns;
     int group = 1;
     while (group < 512 && group * most < runs) group *= 2;
     int per_thread = (runs + group - 1) / group;

@@ -494,3 +494,18 @@ def test_packed_rows_that_four_divides(dim, dtype):
         y64 = ob.rms_norm(x, w)[0]
         _close(add_rms_norm(x, w), y64, dtype)
         _close_quant(*add_rms_norm_quant(x, w), y64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [591, 592, 593])
+def test_wide_rows_around_the_change_of_kernels(rows, dtype):
+    """The count of rows from which blocks walk several of them, without a residual, at widths of three to six runs."""
+    from mindiesd import add_rms_norm, add_rms_norm_quant
+    e = torch.empty(0, dtype=dtype).element_size()
+    for runs in (376, 385, 512, 640, 760, 1536, 1544):
+        dim = runs * 16 // e
+        x, w = _randn(dim, rows, dim, dtype=dtype), _randn(1, dim, dtype=dtype)
+        y64 = ob.rms_norm(x, w)[0]
+        _close(add_rms_norm(x, w), y64, dtype)
+        _close_quant(*add_rms_norm_quant(x, w), y64)
