@@ -530,6 +530,22 @@ typedef struct mindiesd_linear_args {
 int mindiesd_linear_fwd(const mindiesd_linear_args* args, void* stream);
 
 /*
+ * Test hook: the same product cut up as given instead of as chosen from the sizes.
+ *   few_rows = 0: tiles of 256 rows and `tile` columns, a multiple of 32 up to 256 that is less than n + 32; split 1
+ *   few_rows = 1: tiles of 128 columns and `tile` rows, a multiple of 16 up to 128 that is less than m + 16; their k is
+ *                 split over `split` (1 to 8) thread blocks, each with two or more steps of 128 bytes where it is more than 1
+ * blocks_per_sm (few_rows only, else 1): 1 or 2, which is refused where a tile's stages leave no room for it.
+ */
+typedef struct mindiesd_linear_cut {
+    int32_t few_rows;
+    int32_t tile;
+    int32_t split;
+    int32_t blocks_per_sm;
+} mindiesd_linear_cut;
+
+int mindiesd_linear_fwd_as(const mindiesd_linear_args* args, const mindiesd_linear_cut* cut, void* stream);
+
+/*
  * Copies `rows` rows of row_bytes bytes, src_stride bytes apart (0: one row, repeated), to rows dst_stride bytes
  * apart: lays operands out for mindiesd_linear_fwd that do not start on 16 bytes, or that start on 16 but not on
  * 32 bytes (it takes those, but fetches them at a lower rate).  dst and dst_stride are multiples of 16; the bytes from

@@ -1105,6 +1105,20 @@ Plan choose_plan(int m, int n, int k_steps) {
     return c.plan;
 }
 
+// The plan that a test asks for; false where it is none that choose_plan could return for some sizes.
+bool given_plan(const mindiesd_linear_cut& c, int m, int n, int k_steps, Plan& plan) {
+    if (c.few_rows == 0) {
+        if (c.tile < 32 || c.tile > 256 || c.tile % 32 != 0 || c.tile >= static_cast<int64_t>(n) + 32 || c.split != 1 || c.blocks_per_sm != 1) return false;
+        plan = {false, c.tile, pair_stages(c.tile), 1, pair_band(n, k_steps)};
+        return true;
+    }
+    if (c.few_rows != 1 || c.tile < 16 || c.tile > kSwapMaxTile || c.tile % 16 != 0 || c.tile >= static_cast<int64_t>(m) + 16) return false;
+    if (c.split < 1 || c.split > kSwapMaxSplit || (c.split > 1 && k_steps < 2 * c.split)) return false;
+    if (c.blocks_per_sm < 1 || c.blocks_per_sm > 2 || swap_stages(c.tile, c.blocks_per_sm) < 2) return false;
+    plan = {true, c.tile, swap_stages(c.tile, c.blocks_per_sm), c.split, 0};
+    return true;
+}
+
 template <bool kFp8>
 cudaError_t launch_swap(const LinearParams& p, cudaStream_t stream) {
     const dim3 grid(p.split, (p.e.n + 127) / 128, (p.e.m + p.tile_n - 1) / p.tile_n);
@@ -1116,7 +1130,8 @@ cudaError_t launch_swap(const LinearParams& p, cudaStream_t stream) {
 
 using namespace sdb;
 
-extern "C" int mindiesd_linear_fwd(const mindiesd_linear_args* a, void* stream_) try {
+// cut: null, or how a test wants the product cut up.
+static int linear_fwd(const mindiesd_linear_args* a, const mindiesd_linear_cut* cut, void* stream_) try {
     if (!a || !a->x || !a->weight || !a->out) return MINDIESD_E_NULL;
     if (a->m <= 0 || a->n <= 0 || a->k <= 0) return MINDIESD_E_SHAPE;
     if (a->m > 0x7fff0000 || a->n > 0x7fff0000 || a->k > 0x7fff0000) return MINDIESD_E_CAPACITY;  // tile coordinates are 32-bit
@@ -1181,7 +1196,9 @@ extern "C" int mindiesd_linear_fwd(const mindiesd_linear_args* a, void* stream_)
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     int rc;
     cudaError_t err;
-    const Plan plan = choose_plan(a->m, a->n, p.k_steps);
+    Plan plan;
+    if (!cut) plan = choose_plan(a->m, a->n, p.k_steps);
+    else if (!given_plan(*cut, a->m, a->n, p.k_steps, plan)) return MINDIESD_E_VALUE;
     p.tile_n = plan.tile_n;
     p.split = plan.split;
     p.stages = plan.stages;
@@ -1207,4 +1224,10 @@ extern "C" int mindiesd_linear_fwd(const mindiesd_linear_args* a, void* stream_)
     return static_cast<int>(err);
 } catch (...) {  // a lock that the system refused; nothing may cross this boundary
     return MINDIESD_E_DRIVER;
+}
+
+extern "C" int mindiesd_linear_fwd(const mindiesd_linear_args* a, void* stream) { return linear_fwd(a, nullptr, stream); }
+
+extern "C" int mindiesd_linear_fwd_as(const mindiesd_linear_args* a, const mindiesd_linear_cut* cut, void* stream) {
+    return cut ? linear_fwd(a, cut, stream) : MINDIESD_E_NULL;
 }

@@ -166,6 +166,10 @@ class LinearArgs(C.Structure):
     ]
 
 
+class LinearCut(C.Structure):
+    _fields_ = [("few_rows", C.c_int32), ("tile", C.c_int32), ("split", C.c_int32), ("blocks_per_sm", C.c_int32)]
+
+
 class CopyRowsArgs(C.Structure):
     _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("rows", C.c_int64), ("row_bytes", C.c_int64),
                 ("src_stride", C.c_int64), ("dst_stride", C.c_int64)]
@@ -230,6 +234,9 @@ def lib():
             if fn is not None:
                 fn.restype = C.c_int
                 fn.argtypes = [C.c_void_p, C.c_void_p]
+        if hasattr(handle, "mindiesd_linear_fwd_as"):
+            handle.mindiesd_linear_fwd_as.restype = C.c_int
+            handle.mindiesd_linear_fwd_as.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p]
         if hasattr(handle, "mindiesd_rf_block_mask_scratch_bytes"):
             handle.mindiesd_rf_block_mask_scratch_bytes.restype = C.c_size_t
             handle.mindiesd_rf_block_mask_scratch_bytes.argtypes = [C.c_int32] * 4
