@@ -129,7 +129,7 @@ __device__ __forceinline__ float rcp_approx(float x) {
 }
 __device__ __forceinline__ uint64_t both(float v) { return pack2(v, v); }
 
-// v / (1 + 2^x) for a pair; 2^x may be infinite (the quotient is then 0).
+// v / (1 + 2^x) for a pair; the quotient is 0 where 2^x is above 2^126 (the reciprocal flushes there) or infinite.
 __device__ __forceinline__ uint64_t over_one_plus_ex2(uint64_t v, uint64_t x) {
     float lo, hi;
     unpack2(x, lo, hi);
@@ -157,7 +157,8 @@ __device__ __forceinline__ uint64_t gelu_pair(uint64_t v) {
     return fma2(mul2(a, both(-0.5f)), q, pack2(lo < 0.0f ? 0.0f : lo, hi < 0.0f ? 0.0f : hi));  // a NaN stays
 }
 
-// The activations, on pairs of values, in the forms that keep their relative accuracy for large negative arguments:
+// The activations, on pairs of values, in the forms that keep their relative accuracy for large negative arguments, down to
+// values of |v| 2^-126, which become 0 (silu below -87.3, gelu below -13.2, gelu_tanh below -10.0):
 //   gelu(v) = v/2 erfc(-v / sqrt 2) (gelu_pair),  silu(v) = v / (1 + e^-v),
 //   gelu_tanh(v) = v/2 (1 + tanh u) = v / (1 + e^-2u),  u = sqrt(2/pi) (v + 0.044715 v^3).
 template <int kPairs>

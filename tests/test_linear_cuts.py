@@ -9,6 +9,7 @@ import torch
 
 import test_linear_forward as tl
 from mindiesd import _cabi
+from oracle import block_linear as ob
 
 PAIR = [(0, tile, 1, 1) for tile in range(32, 257, 32)]
 SWAP = [(1, tile, split, per_sm) for tile in range(16, 129, 16) for split in range(1, 9) for per_sm in (1, 2)
@@ -233,3 +234,22 @@ def test_at_once_captured_and_replayed(cut):
     x.copy_(tl._randn(52, m, k, dtype=torch.bfloat16))
     graph.replay()
     assert torch.equal(captured, call())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cut", [(0, 96, 1, 1), (1, 32, 2, 1)])
+@pytest.mark.parametrize("act", ["relu", "silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_activations_relative_accuracy(cut, act, dtype):
+    """The other operand is the unit matrix, so a sum is one product and exact, and the tolerance is the activation's alone: its
+    2^-15 and the last rounding, both relative, and |v| 2^-126, where the reciprocal and the exponential flush to zero."""
+    n = 256
+    eye = torch.eye(n, dtype=dtype, device="cuda")
+    edge = {"relu": 1.0, "silu": 87.34, "gelu": 13.22, "gelu_tanh": 10.0}[act]
+    v = torch.cat([torch.linspace(-1.2 * edge, 0, 40 * n, device="cuda"), torch.linspace(-1.05 * edge, -0.95 * edge, 20 * n, device="cuda"),
+                   torch.linspace(0, 100, 20 * n, device="cuda"), -torch.logspace(-4, 2, 20 * n, device="cuda")]).to(dtype).view(-1, n)
+    out = _run(cut, v, eye, torch.empty(v.shape, dtype=dtype, device="cuda"), act=act)
+    want = ob.activation(v.double(), act)
+    tol = want.abs() * (ob.half_step(dtype) + tl.ACT_SLACK) + ob.smallest_half_step(dtype) + v.double().abs() * 2.0 ** -126
+    worst = ((out.double() - want).abs() - tol).max().item()
+    assert worst <= 0, worst
