@@ -5,8 +5,9 @@ with NaN and set a per-device status word; while the word is set, later launches
 at once and mark their rows too.  Reading the word synchronises the device, so the layer API does it
 only where it synchronises anyway (the host-operand entry points) or when asked to:
 
-    MINDIESD_CHECK_STATUS=1   attention_forward, sparse_attention, attention_forward_varlen and
-                              FP8RotateQuantFA read the word after every call and raise ModelExecError
+    MINDIESD_CHECK_STATUS=1   attention_forward, sparse_attention, attention_forward_varlen,
+                              FP8RotateQuantFA, linear_forward and FP8DynamicLinear read the word after every call
+                              and raise ModelExecError
 """
 import os
 
