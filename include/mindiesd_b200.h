@@ -438,7 +438,7 @@ int mindiesd_rope(const mindiesd_rope_args* args, void* stream);
 
 /*
  * Residual addition, root-mean-square norm and per-token quantisation of [rows, dim] activations:
- *   v = x + residual (fp32),  y = v * weight / sqrt(mean(v^2) + eps)  (fp32)
+ *   v = x + residual (fp32),  y = v * weight / sqrt(mean(v^2) + eps)  (fp32, in this order: v * weight has to be in range)
  *   out          = y rounded once to the type of x, or e4m3 of y / scale (out_dtype = MINDIESD_E4M3)
  *   scales       fp32 [rows], e4m3 only: max|y| / 448 of the row (at least 2^-126), 1 for a row of zeros;
  *                real value = stored value * scale.  A NaN or infinity in a row makes its scale NaN
